@@ -1,0 +1,291 @@
+"""torch bindings of include/mgrid_norm.h: layer norm with its gradients, and clipping by the global gradient norm, both in
+the trainer's stacked form too (every tensor with a leading agent axis, one weight row and one norm per agent).
+
+`layer_norm(x, weight, bias)` is what the policies call with `layer_norm=True`; `clip_grad_norm_` is the clipping of an update
+epoch (v8_robust_ppo.py:340).  `clip_grads` is the same clipping into other tensors, `grad_norm` the norm alone.  On a GPU
+they run the HIP kernels of libmgnn.so on the current stream, for float32, bfloat16 and float16 (a missing library raises);
+CPU tensors take the plain torch expression of the same formulas.  What neither takes is refused with a TypeError (types,
+layouts) or a ValueError (shapes, sizes, devices, overlapping memory) before anything is written.
+
+Nothing is kept between calls: workspaces come from torch's allocator, so every captured graph has its own.
+"""
+import array
+import ctypes as C
+import math
+
+import torch
+import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
+
+from . import fused_ops
+
+MAX_COLS = 16384      # MGNN_LN_MAX_C
+MAX_GROUPS = 65535    # MGNN_MAX_GROUPS
+TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+# name -> (restype, argtypes): every symbol include/mgrid_norm.h declares
+SYMBOLS = {
+    'mgnn_layer_norm': (C.c_int, [C.c_void_p, C.c_int64] + [C.c_void_p] * 4 + [C.c_int64, C.c_int64, C.c_int, C.c_double, C.c_int, C.c_int,
+                                                                            C.c_void_p]),
+    'mgnn_layer_norm_workspace': (C.c_int64, [C.c_int64, C.c_int64, C.c_int, C.c_int]),
+    'mgnn_layer_norm_backward': (C.c_int, [C.c_void_p, C.c_int64] + [C.c_void_p] * 7 + [C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int,
+                                                                                     C.c_int, C.c_void_p]),
+    'mgnn_grad_norm_workspace': (C.c_int64, [C.c_void_p, C.c_void_p, C.c_int64, C.c_int64]),
+    'mgnn_grad_norm': (C.c_int, [C.c_void_p] * 3 + [C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    'mgnn_clip_grads': (C.c_int, [C.c_void_p] * 4 + [C.c_int64, C.c_int64, C.c_double, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+}
+ERRORS = {1: 'a size is out of range', 2: 'the kernel launch failed', 3: 'an element type is not supported', 4: 'the workspace does not fit',
+          5: 'an argument is invalid', 6: 'a gradient that is written overlaps another one'}
+_LIB = None
+
+
+def load():
+  global _LIB
+  if _LIB is None:
+    fused_ops.load()      # raises if libmgnn.so is missing
+    lib = C.CDLL(fused_ops.LIB_PATH)
+    for name, (res, args) in SYMBOLS.items():
+      fn = getattr(lib, name)
+      fn.restype, fn.argtypes = res, args
+    _LIB = lib
+  return _LIB
+
+
+def _check(rc, what):
+  if rc != 0:
+    raise (RuntimeError if rc == 2 else ValueError)('%s: %s (MGNN error %d)' % (what, ERRORS.get(rc, 'unknown'), rc))
+
+
+def _stream(dev):
+  return torch.cuda.current_stream(dev).cuda_stream
+
+
+# ---- layer norm ----
+
+def _ln_args(x, weight, bias, eps):
+  """The number of weight rows (1, or the leading axis of x)."""
+  if x.dtype not in TYPES or x.layout != torch.strided:
+    raise TypeError('layer_norm takes dense float32, bfloat16 or float16 tensors, not %s' % x.dtype)
+  if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_COLS:
+    raise ValueError('layer_norm takes rows of 1 to %d elements, not a tensor of shape %s' % (MAX_COLS, tuple(x.shape)))
+  if not eps >= 0 or math.isinf(eps):
+    raise ValueError('layer_norm takes a finite eps >= 0, not %r' % (eps,))
+  groups = 1
+  for name, t in (('weight', weight), ('bias', bias)):
+    if t is None:
+      continue
+    if t.dtype not in (x.dtype, torch.float32) or t.layout != torch.strided:
+      raise TypeError("layer_norm's %s is %s: x's type (%s) or float32 is wanted" % (name, t.dtype, x.dtype))
+    if t.device != x.device:
+      raise ValueError("layer_norm's %s is on %s, x on %s" % (name, t.device, x.device))
+    stacked = t.dim() == 2 and x.dim() >= 2 and t.shape[0] == x.shape[0]
+    if t.shape[-1:] != x.shape[-1:] or not (t.dim() == 1 or stacked):
+      raise ValueError("layer_norm's %s of shape %s does not fit x of shape %s: [cols] or [x.shape[0], cols] is wanted"
+                       % (name, tuple(t.shape), tuple(x.shape)))
+    groups = t.shape[0] if stacked else 1
+  if weight is not None and bias is not None and (weight.shape != bias.shape or weight.dtype != bias.dtype):
+    raise ValueError("layer_norm's weight and bias differ in shape or type")
+  if groups > MAX_GROUPS:
+    raise ValueError('layer_norm takes at most %d weight rows, not %d' % (MAX_GROUPS, groups))
+  return groups
+
+
+def _rows(x):
+  """x as [rows, cols] with contiguous rows at one distance (a view where there is one), and that distance."""
+  cols = x.shape[-1]
+  n = x.numel() // cols
+  x2 = x.reshape(n, cols)
+  if (cols > 1 and x2.stride(1) != 1) or (n > 1 and x2.stride(0) < cols):
+    x2 = x2.contiguous()
+  return x2, x2.stride(0) if n > 1 else cols
+
+
+def _ptr(t):
+  return None if t is None else t.data_ptr()
+
+
+def _ln_forward(x, weight, bias, eps, groups, want_stats):
+  dev = x.device
+  x2, ld = _rows(x)
+  n, cols = x2.shape
+  weight = None if weight is None else weight.contiguous()
+  bias = None if bias is None else bias.contiguous()
+  wt = weight if weight is not None else bias
+  y = torch.empty(x.shape, dtype=x.dtype, device=dev)
+  stats = torch.empty((n, 2), dtype=torch.float32, device=dev) if want_stats else None
+  with torch.cuda.device(dev):
+    _check(load().mgnn_layer_norm(x2.data_ptr(), ld, _ptr(weight), _ptr(bias), y.data_ptr(), _ptr(stats), groups,
+                                  n // groups if groups else 0, cols, eps, TYPES[x.dtype], TYPES[x.dtype if wt is None else wt.dtype],
+                                  _stream(dev)), 'mgnn_layer_norm')
+  return y, x2, stats, weight
+
+
+class _LayerNorm(torch.autograd.Function):
+
+  @staticmethod
+  def forward(ctx, x, weight, bias, eps, groups):
+    y, x2, stats, w = _ln_forward(x, weight, bias, eps, groups, True)
+    ctx.save_for_backward(x2, stats, w)
+    ctx.groups, ctx.shape = groups, x.shape
+    ctx.affine = [None if t is None else (t.shape, t.dtype) for t in (weight, bias)]
+    return y
+
+  @staticmethod
+  @once_differentiable
+  def backward(ctx, dy):
+    x2, stats, w = ctx.saved_tensors
+    want_x, want_w, want_b = ctx.needs_input_grad[:3]
+    dev, groups = x2.device, ctx.groups
+    n, cols = x2.shape
+    rows = n // groups if groups else 0
+    dy = dy.contiguous()
+    dx = torch.empty(ctx.shape, dtype=x2.dtype, device=dev) if want_x else None
+    dw, db = (torch.empty(s[0], dtype=s[1], device=dev) if want else None
+              for want, s in ((want_w, ctx.affine[0]), (want_b, ctx.affine[1])))
+    wt = next((s[1] for s in ctx.affine if s is not None), x2.dtype)
+    lib = load()
+    size = lib.mgnn_layer_norm_workspace(groups, rows, cols, TYPES[x2.dtype]) if want_w or want_b else 0
+    room = torch.empty(size // 4, dtype=torch.float32, device=dev) if size > 0 else None
+    with torch.cuda.device(dev):
+      _check(lib.mgnn_layer_norm_backward(x2.data_ptr(), x2.stride(0) if n > 1 else cols, dy.data_ptr(), _ptr(w), stats.data_ptr(),
+                                          _ptr(dx), _ptr(dw), _ptr(db), _ptr(room), size, groups, rows, cols, TYPES[x2.dtype],
+                                          TYPES[wt], _stream(dev)), 'mgnn_layer_norm_backward')
+    return dx, dw, db, None, None
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5):
+  """Layer norm over the last axis: (x - mean) / sqrt(mean((x - mean)^2) + eps) * weight + bias, in x's type, with the
+  statistics and every sum in float32.  weight / bias: [cols] of x's type or float32, or None; [x.shape[0], cols] gives
+  every index of x's leading axis (an agent) its own.  Rows of 1 to 16384 elements.  Differentiable once in all three."""
+  groups = _ln_args(x, weight, bias, eps)
+  if x.is_cuda:
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
+      return _LayerNorm.apply(x, weight, bias, eps, groups)
+    return _ln_forward(x, weight, bias, eps, groups, False)[0]
+  h = F.layer_norm(x.float(), x.shape[-1:], None, None, eps)
+  wide = (x.shape[0],) + (1,) * (x.dim() - 2) + x.shape[-1:]      # a stacked weight against x
+  if weight is not None:
+    h = h * (weight.float().reshape(wide) if weight.dim() == 2 else weight.float())
+  if bias is not None:
+    h = h + (bias.float().reshape(wide) if bias.dim() == 2 else bias.float())
+  return h.to(x.dtype)
+
+
+# ---- the global gradient norm ----
+
+def _dense(t, stacked):
+  """Whether t's elements fill one stretch of memory, in whatever order (stacked: agent by agent)."""
+  if t.is_contiguous():
+    return True
+  order = sorted(range(t.dim()), key=lambda d: (t.stride(d), d == 0), reverse=True)
+  return t.permute(order).is_contiguous() and (not stacked or order[0] == 0)
+
+
+def _grad_list(grads, stacked):
+  grads = [grads] if isinstance(grads, torch.Tensor) else list(grads)
+  if not isinstance(stacked, int) or not 0 <= stacked <= MAX_GROUPS:
+    raise ValueError('stacked is the length of the leading agent axis, 0 (none) to %d, not %r' % (MAX_GROUPS, stacked))
+  dev = grads[0].device if grads else None
+  for g in grads:
+    if g.dtype not in TYPES or g.layout != torch.strided:
+      raise TypeError('gradients are dense float32, bfloat16 or float16 tensors, not %s, %s' % (g.dtype, g.layout))
+    if g.device != dev:
+      raise ValueError('gradients are on %s and %s: one device is wanted' % (dev, g.device))
+    if stacked and (g.dim() < 1 or g.shape[0] != stacked):
+      raise ValueError('a gradient of shape %s has no leading agent axis of %d' % (tuple(g.shape), stacked))
+  return grads, dev
+
+
+def takes(grads):
+  """Whether grads, a list, are what the kernels take: tensors on a GPU, of the types they know."""
+  return bool(grads) and all(g.is_cuda and g.dtype in TYPES and g.layout == torch.strided for g in grads)
+
+
+def _address(a):
+  return a.buffer_info()[0]
+
+
+def _launch(src, dst, max_norm, stacked, dev):
+  """The kernels on dense tensors; dst None: the norms alone."""
+  lib, groups = load(), stacked or 1
+  count = len(src)
+  n = array.array('q', [t.numel() // groups for t in src])
+  types = array.array('i', [TYPES[t.dtype] for t in src])
+  sp = array.array('Q', [t.data_ptr() for t in src])
+  norms = torch.empty((stacked,) if stacked else (), dtype=torch.float32, device=dev)
+  size = lib.mgnn_grad_norm_workspace(_address(n), _address(types), count, groups)
+  room = torch.empty(size // 8, dtype=torch.float64, device=dev) if size > 0 else None
+  with torch.cuda.device(dev):
+    if dst is None:
+      _check(lib.mgnn_grad_norm(_address(sp), _address(n), _address(types), count, groups, norms.data_ptr(), _ptr(room), size,
+                                _stream(dev)), 'mgnn_grad_norm')
+    else:
+      dp = array.array('Q', [t.data_ptr() for t in dst])
+      _check(lib.mgnn_clip_grads(_address(sp), _address(dp), _address(n), _address(types), count, groups, max_norm, norms.data_ptr(),
+                                 _ptr(room), size, _stream(dev)), 'mgnn_clip_grads')
+  return norms
+
+
+def _plain_norms(grads, stacked):
+  if not grads:
+    return torch.zeros((stacked,) if stacked else ())
+  sq = sum(g.double().reshape(stacked or 1, -1).square().sum(dim=1) for g in grads)
+  return sq.sqrt() if stacked else sq.sqrt()[0]
+
+
+@torch.no_grad()
+def grad_norm(grads, stacked=0):
+  """The 2-norm of all gradients together, a float32 scalar on their device; stacked=A: every gradient has a leading
+  agent axis of A, and agent a's norm is element a of the result.  Squares are added in float64.  No gradients: 0."""
+  grads, dev = _grad_list(grads, stacked)
+  if dev is None or dev.type != 'cuda':
+    return _plain_norms(grads, stacked).float()
+  return _launch([g if _dense(g, stacked) else g.contiguous() for g in grads], None, 0.0, stacked, dev)
+
+
+@torch.no_grad()
+def clip_grads(grads, max_norm, stacked=0, out=None):
+  """([g * min(1, max_norm / (norm + 1e-6)) for every gradient g], norm) with norm = grad_norm(grads, stacked); agent by
+  agent if stacked.  out: tensors of the gradients' shapes and types that receive the results (the gradients themselves:
+  in place); none of them may overlap another gradient of the call.  A norm that is NaN makes every result NaN."""
+  grads, dev = _grad_list(grads, stacked)
+  max_norm = float(max_norm)
+  if not max_norm >= 0:
+    raise ValueError('max_norm is a number >= 0, not %r' % max_norm)
+  if out is None:
+    out = [torch.empty_like(g) for g in grads]
+  else:
+    out = list(out)
+    if len(out) != len(grads) or any(o.shape != g.shape or o.dtype != g.dtype or o.device != g.device for o, g in zip(out, grads)):
+      raise ValueError('out does not match the gradients in number, shape, type or device')
+    if any(0 in [s for s, k in zip(o.stride(), o.shape) if k > 1] for o in out if not o.is_contiguous()):
+      raise ValueError('a gradient that is written has several elements at one address (an expanded tensor)')
+  if dev is None or dev.type != 'cuda':
+    norms = _plain_norms(grads, stacked)
+    factor = (max_norm / (norms + 1e-6)).clamp(max=1.0).float()
+    for o, g in zip(out, grads):
+      o.copy_(g.float() * factor.reshape(factor.shape + (1,) * (g.dim() - factor.dim())))
+    return out, norms.float()
+  src, dst = [], []
+  for g, o in zip(grads, out):
+    if g.is_contiguous() and o.is_contiguous() or (g.stride() == o.stride() and _dense(g, stacked)):
+      src.append(g)
+      dst.append(o)
+    else:      # no common dense order: through contiguous copies
+      src.append(g.contiguous())
+      dst.append(src[-1] if o is g else torch.empty(o.shape, dtype=o.dtype, device=dev))
+  norms = _launch(src, dst, max_norm, stacked, dev)
+  torch.autograd.graph.increment_version(dst)      # written behind autograd's back: a graph that saved one of them will say so
+  for d, o in zip(dst, out):
+    if d is not o:
+      o.copy_(d)
+  return out, norms
+
+
+def clip_grad_norm_(parameters, max_norm, stacked=0):
+  """torch.nn.utils.clip_grad_norm_ (v8_robust_ppo.py:340) on the parameters' .grad in place; parameters without one are
+  left out.  stacked=A: agent by agent.  Returns the norm(s) before clipping."""
+  parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
+  grads = [p.grad for p in parameters if p.grad is not None]
+  return clip_grads(grads, max_norm, stacked, out=grads)[1]

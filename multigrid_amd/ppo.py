@@ -1,6 +1,6 @@
 """Batched v8 PPO on top of the device-resident env.
 
-PyTorch-ROCm only (no HIP kernels here): the policy consumes `env.obs_image` / `env.obs_dir` in place, writes its
+PyTorch-ROCm and the trainer's own HIP operators (fused_ops.py, norm_ops.py): the policy consumes `env.obs_image` / `env.obs_dir` in place, writes its
 sampled actions into `env.actions`, and `env.step()` is one kernel launch on the same stream — no host round trip per
 step, where the reference does 3 batch-1 forwards with an `.item()` sync each (v8_robust_ppo.py:138-157).
 
@@ -25,13 +25,14 @@ from torch import nn
 from torch.distributions import Categorical
 import torch.nn.functional as F
 
-from . import fused_ops
+from . import fused_ops, norm_ops
 
 
 class AgentNet(nn.Module):
-  """SimplePPOAgent (v8_robust_ppo.py:35-102), batch-first only."""
+  """SimplePPOAgent (v8_robust_ppo.py:35-102), batch-first only.  layer_norm=True (not in the reference): a layer norm
+  between each hidden linear layer and its ReLU; every other parameter keeps its name."""
 
-  def __init__(self, n_actions=7):
+  def __init__(self, n_actions=7, layer_norm=False):
     super().__init__()
     self.image_conv = nn.Sequential(
         nn.Conv2d(3, 32, 3, padding=1), nn.ReLU(),
@@ -45,12 +46,17 @@ class AgentNet(nn.Module):
       if isinstance(m, nn.Linear):
         nn.init.orthogonal_(m.weight, 0.5)
         m.bias.data.zero_()
+    self.norms = nn.ModuleList([nn.LayerNorm(128), nn.LayerNorm(64)]) if layer_norm else None
 
   def forward(self, image, direction):
     """image: uint8/float [B, V, V, 3] laid out [x][y][c] as the env writes it; direction: [B]."""
     x = image.permute(0, 3, 1, 2).float()          # v8:75 — channels first, x/y kept as they are
     feat = torch.cat([self.image_conv(x), self.direction_embed(direction.long())], dim=-1)
-    h = self.shared(feat)
+    if self.norms is None:
+      h = self.shared(feat)
+    else:
+      h = F.relu(self.norms[0](self.shared[0](feat)))
+      h = F.relu(self.norms[1](self.shared[2](h)))
     return self.actor(h), self.critic(h).squeeze(-1)
 
   def get_action_and_value(self, image, direction, action=None):
@@ -128,6 +134,9 @@ _STACK = (('image_conv.0.weight', 'conv1_w', (32, 3, 3, 3)), ('image_conv.0.bias
           ('shared.2.weight', 'fc2_w', (64, 128)), ('shared.2.bias', 'fc2_b', (64,)),
           ('actor.weight', 'actor_w', (7, 64)), ('actor.bias', 'actor_b', (7,)),
           ('critic.weight', 'critic_w', (1, 64)), ('critic.bias', 'critic_b', (1,)))
+# and those of layer_norm=True
+_STACK_NORMS = (('norms.0.weight', 'norm1_w', (128,)), ('norms.0.bias', 'norm1_b', (128,)),
+                ('norms.1.weight', 'norm2_w', (64,)), ('norms.1.bias', 'norm2_b', (64,)))
 
 
 class StackedAgentNets(nn.Module):
@@ -137,32 +146,38 @@ class StackedAgentNets(nn.Module):
   convolutions per agent (conv_mode='loop', the default: exactly the two conv shapes of the reference net, which MIOpen
   serves at once) or as ONE grouped convolution (conv_mode='grouped', groups = A: agent a's channels only ever meet agent
   a's filters — fewer launches, but a shape MIOpen compiles for minutes on a fresh box before its first call returns).
-  Mathematically both are exactly A separate nets: gradients of a summed loss do not mix agents."""
+  Mathematically both are exactly A separate nets: gradients of a summed loss do not mix agents.
 
-  def __init__(self, n_agents, n_actions=7, conv_mode='loop'):
+  layer_norm=True (not in the reference): each hidden layer's pre-activations of all agents pass one stacked layer norm
+  (norm_ops.layer_norm, csrc/norm_ops.hip on a GPU) before the ReLU."""
+
+  def __init__(self, n_agents, n_actions=7, conv_mode='loop', layer_norm=False):
     super().__init__()
-    self.n_agents, self.n_actions, self.conv_mode = n_agents, n_actions, conv_mode
-    nets = [AgentNet(n_actions) for _ in range(n_agents)]        # the reference's initialisation, agent by agent
-    for ref_name, name, _ in _STACK:
+    self.n_agents, self.n_actions, self.conv_mode, self.layer_norm = n_agents, n_actions, conv_mode, layer_norm
+    self.stack = _STACK + (_STACK_NORMS if layer_norm else ())
+    nets = [AgentNet(n_actions, layer_norm) for _ in range(n_agents)]        # the reference's initialisation, agent by agent
+    for ref_name, name, _ in self.stack:
       self.register_parameter(name, nn.Parameter(torch.stack([n.state_dict()[ref_name] for n in nets]).contiguous()))
 
   def agent_state_dict(self, a):
     """Agent a's weights under the reference's names (what SimplePPOAgent.state_dict() holds)."""
-    return {ref_name: getattr(self, name)[a].detach().clone() for ref_name, name, _ in _STACK}
+    return {ref_name: getattr(self, name)[a].detach().clone() for ref_name, name, _ in self.stack}
 
   def load_agent_state_dict(self, a, sd):
+    if ('norms.0.weight' in sd) != self.layer_norm:
+      raise ValueError('weights %s layer norms do not fit a policy %s them' % (('without', 'with') if self.layer_norm else ('with', 'without')))
     with torch.no_grad():
-      for ref_name, name, shape in _STACK:
+      for ref_name, name, shape in self.stack:
         getattr(self, name)[a].copy_(sd[ref_name].reshape(shape))
 
   def agent_net(self, a):
     """A stand-alone AgentNet holding a COPY of agent a's weights."""
-    net = AgentNet(self.n_actions)
+    net = AgentNet(self.n_actions, self.layer_norm)
     net.load_state_dict(self.agent_state_dict(a))
     return net.to(self.conv1_w.device)
 
   def agent_parameters(self, a):
-    return [getattr(self, name)[a] for _, name, _ in _STACK]
+    return [getattr(self, name)[a] for _, name, _ in self.stack]
 
   def forward(self, image, direction):
     """image [A, B, V, V, 3] (uint8 or float, [x][y][c] as the env writes it), direction [A, B] ->
@@ -184,20 +199,27 @@ class StackedAgentNets(nn.Module):
     idx = direction.long().unsqueeze(-1).expand(A, B, 8)
     emb = torch.gather(self.embed, 1, idx)                                  # direction_embed, per agent
     h = torch.cat([feat, emb], dim=-1)                                      # [A, B, 72]
-    h = F.relu(torch.baddbmm(self.fc1_b.unsqueeze(1), h, self.fc1_w.transpose(1, 2)))
-    h = F.relu(torch.baddbmm(self.fc2_b.unsqueeze(1), h, self.fc2_w.transpose(1, 2)))
+    h = torch.baddbmm(self.fc1_b.unsqueeze(1), h, self.fc1_w.transpose(1, 2))
+    h = F.relu(norm_ops.layer_norm(h, self.norm1_w, self.norm1_b) if self.layer_norm else h)
+    h = torch.baddbmm(self.fc2_b.unsqueeze(1), h, self.fc2_w.transpose(1, 2))
+    h = F.relu(norm_ops.layer_norm(h, self.norm2_w, self.norm2_b) if self.layer_norm else h)
     logits = torch.baddbmm(self.actor_b.unsqueeze(1), h, self.actor_w.transpose(1, 2))
     values = torch.baddbmm(self.critic_b.unsqueeze(1), h, self.critic_w.transpose(1, 2)).squeeze(-1)
     return logits, values
 
   def clip_grad_norm_(self, max_norm):
-    """torch.nn.utils.clip_grad_norm_(agent.parameters(), max_norm) (v8:340) for every agent separately."""
-    grads = [getattr(self, name).grad for _, name, _ in _STACK]
-    sq = sum(g.reshape(self.n_agents, -1).pow(2).sum(dim=1) for g in grads if g is not None)
-    coef = (max_norm / (sq.sqrt() + 1e-6)).clamp(max=1.0)
+    """torch.nn.utils.clip_grad_norm_(agent.parameters(), max_norm) (v8:340) for every agent separately; returns the
+    agents' norms.  On a GPU one pass of csrc/norm_ops.hip over all agents' gradients."""
+    grads = [getattr(self, name).grad for _, name, _ in self.stack]
+    grads = [g for g in grads if g is not None]
+    if norm_ops.takes(grads):
+      return norm_ops.clip_grads(grads, max_norm, stacked=self.n_agents, out=grads)[1]
+    sq = sum(g.reshape(self.n_agents, -1).pow(2).sum(dim=1) for g in grads)
+    norms = sq.sqrt()
+    coef = (max_norm / (norms + 1e-6)).clamp(max=1.0)
     for g in grads:
-      if g is not None:
-        g.mul_(coef.reshape((-1,) + (1,) * (g.dim() - 1)))
+      g.mul_(coef.reshape((-1,) + (1,) * (g.dim() - 1)))
+    return norms
 
 
 class PerAgentNets(nn.Module):
@@ -228,7 +250,11 @@ class PerAgentNets(nn.Module):
 
   def clip_grad_norm_(self, max_norm):
     for net in self.nets:
-      torch.nn.utils.clip_grad_norm_(net.parameters(), max_norm)
+      grads = [p.grad for p in net.parameters() if p.grad is not None]
+      if norm_ops.takes(grads):
+        norm_ops.clip_grads(grads, max_norm, out=grads)
+      else:
+        torch.nn.utils.clip_grad_norm_(net.parameters(), max_norm)
 
 
 def compute_gae(rewards, values, dones, gamma=0.99, gae_lambda=0.95):
@@ -378,9 +404,10 @@ class BatchedController:
   and its reducer, driving gloo on device buckets from autograd's hooks, is where the two-rank rehearsal on one GPU
   stood still in round 2 (both ranks inside loss.backward()).  amp=torch.bfloat16 runs the update's forward / backward under autocast — NOT the
   reference's precision (fp32, the default here); it exists to show what the matrix cores would buy.
+  layer_norm=True puts a layer norm behind each hidden linear layer of policy='simple' (the reference has none).
   """
 
-  def __init__(self, env, lr=1e-4, device=None, ddp=None, seed=0, policy='simple', conv_mode='loop', amp=None):
+  def __init__(self, env, lr=1e-4, device=None, ddp=None, seed=0, policy='simple', conv_mode='loop', amp=None, layer_norm=False):
     self.env = env
     self.n_agents = A = env.n_agents
     self.device = device if device is not None else env.obs_image.device
@@ -389,8 +416,10 @@ class BatchedController:
     distributed = dist.is_available() and dist.is_initialized() and dist.get_world_size() > 1
     torch.manual_seed(seed)                       # same initial weights on every rank
     if policy == 'simple':
-      self.policy = StackedAgentNets(A, conv_mode=conv_mode).to(self.device)
+      self.policy = StackedAgentNets(A, conv_mode=conv_mode, layer_norm=layer_norm).to(self.device)
     elif policy == 'multigrid_net':
+      if layer_norm:
+        raise ValueError("layer_norm is for policy='simple'")
       self.policy = PerAgentNets([MultiGridPPONet(n_agents=A) for _ in range(A)], all_dirs=True).to(self.device)
     else:
       raise ValueError('policy must be "simple" or "multigrid_net"')

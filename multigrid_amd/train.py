@@ -30,6 +30,7 @@ def main(argv=None):
   ap.add_argument('--no-graph', action='store_true')
   ap.add_argument('--policy', default='simple', choices=['simple', 'multigrid_net'],
                   help="simple = v8's SimplePPOAgent per agent; multigrid_net = networks/multigrid_network.py per agent (+ value head)")
+  ap.add_argument('--layer-norm', action='store_true', help='a layer norm behind each hidden linear layer (policy simple; the reference has none)')
   ap.add_argument('--backend', default='nccl', help='torch.distributed backend when several ranks run (nccl = RCCL); gloo to rehearse')
   ap.add_argument('--all-on-device0', action='store_true', help='rehearsal: every rank uses cuda:0')
   ap.add_argument('--dump-weights', default=None, help='write this rank\'s final policy state_dict to <path>.rank<r>.pt (tests)')
@@ -74,7 +75,8 @@ def main(argv=None):
                                    shaping='v8', auto_reset=True)
   env.reset()
   stage('process group and envs up')
-  ctl = ppo.BatchedController(env, lr=args.lr, seed=args.seed, policy=args.policy, ddp=False if args.no_ddp else None)
+  ctl = ppo.BatchedController(env, lr=args.lr, seed=args.seed, policy=args.policy, ddp=False if args.no_ddp else None,
+                              layer_norm=args.layer_norm)
   stage('controller built (gradient all-reduce: %s)' % ctl.ddp)
   window, best = [], float('-inf')
   t0 = time.time()
