@@ -6,6 +6,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 #include <utility>
 #include <vector>
 
@@ -48,130 +49,200 @@ __device__ __forceinline__ void store_part(T* row, int col, int C, typename Pack
   }
 }
 
-__device__ __forceinline__ float load_as_float(const void* p, int type, int64_t i) {
-  if (type == MGNN_F32) return static_cast<const float*>(p)[i];
-  if (type == MGNN_BF16) return (float)static_cast<const __bf16*>(p)[i];
-  return (float)static_cast<const _Float16*>(p)[i];
-}
-
 __device__ __forceinline__ void store_from_float(void* p, int type, int64_t i, float v) {
   if (type == MGNN_F32) static_cast<float*>(p)[i] = v;
   else if (type == MGNN_BF16) static_cast<__bf16*>(p)[i] = (__bf16)v;
   else static_cast<_Float16*>(p)[i] = (_Float16)v;
 }
 
-// sum over aligned groups of L lanes, in every lane of the group (all 64 lanes take part)
+// Sum over aligned groups of L lanes, in every lane of the group (all 64 lanes take part), on the vector units alone: lane
+// permutations within 16 lanes, then whole rows of 16 and halves of the wave swapped between two registers.
+template <int CTRL>
+__device__ __forceinline__ float dpp_add(float v) {
+  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
 template <int L>
 __device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int s = 1; s < L; s <<= 1) v += __shfl_xor(v, s);
+  if constexpr (L >= 2) v = dpp_add<0xB1>(v);       // lane ^ 1
+  if constexpr (L >= 4) v = dpp_add<0x4E>(v);       // lane ^ 2
+  if constexpr (L >= 8) v = dpp_add<0x141>(v);      // mirrored within 8: the other four lanes
+  if constexpr (L >= 16) v = dpp_add<0x140>(v);     // mirrored within 16: the other eight
+  if constexpr (L >= 32) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
+  if constexpr (L >= 64) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  }
   return v;
 }
 
 // ---- layer norm ----
 // TPR threads share a row, thread t holding the vectors t, t + TPR, ... (NV of them) in registers, so a row is read once;
-// a workgroup works on SLOTS rows at a time.  Rows of up to 64 vectors belong to part of a wave or a whole one and need no
-// barrier; longer ones to a whole workgroup.
+// a workgroup works on SLOTS rows at a time.  Rows of up to 64 * NV vectors belong to part of a wave or a whole one and need
+// no barrier; longer ones to several waves.
 template <int TPR>
 struct Shape {
   static constexpr int BLOCK = TPR > 256 ? TPR : 256;
   static constexpr int SLOTS = BLOCK / TPR;
   static constexpr int WAVES = BLOCK / kWave;
+  static constexpr int L = TPR < kWave ? TPR : kWave;              // lanes of a wave that share a row
   static constexpr int ROW_WAVES = TPR > kWave ? TPR / kWave : 1;
 };
 
-// Mean and sum of squared deviations of a row whose elements the TPR threads hold (those past C are not counted): two
-// passes over the registers, so no digits cancel.  Rows over several waves: each wave's own mean and deviations, combined
-// as M = sum M_w + n_w (m_w - m)^2, which takes one barrier instead of two.
-template <int TPR, int NE, int V>
-__device__ __forceinline__ void row_stats(const float (&v)[NE], int lane, int C, float2 (*red)[Shape<TPR>::WAVES], int parity,
-                                          float& mean, float& m2) {
-  constexpr int L = TPR < kWave ? TPR : kWave;
+// Where a thread's vectors lie in a row of C elements.  FULL: the row is exactly TPR * NV vectors.  Else the last vector of
+// a row whose length is no multiple of V ends at the row's end and overlaps the one before by `dup` elements, which it
+// loads and stores like the rest (both threads compute the same values) but leaves out of sums; rows shorter than one
+// vector are moved element by element.  With several vectors per thread the row is longer than half of TPR * NV vectors
+// (row_split), so the first half of them lies inside it.
+template <typename T, int TPR, int NV, bool FULL>
+struct Cols {
+  static constexpr int V = Pack<T>::V;
+  int at[NV], dup[NV];      // first column, leading elements that another thread counts (V: no vector)
+  int C;
+  __device__ __forceinline__ Cols(int lane, int C_) : C(C_) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      const int col = (lane + i * TPR) * V;
+      at[i] = inside(i) ? col : max(min(col, C - V), 0);
+      dup[i] = inside(i) ? 0 : min(col - at[i], V);
+    }
+  }
+  static __device__ __forceinline__ constexpr bool inside(int i) { return FULL || i < NV / 2; }
+  // whether element k of vector i counts (a vector that ends past C starts at column 0 of a row shorter than itself)
+  __device__ __forceinline__ bool counts(int i, int k) const { return inside(i) || (k >= dup[i] && (NV > 1 || k < C)); }
+  __device__ __forceinline__ int count() const {
+    if (FULL) return NV * V;
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) n += max(min(V, C) - dup[i], 0);
+    return n;
+  }
+  __device__ __forceinline__ void load(const T* row, bool live, typename Pack<T>::Vec (&v)[NV]) const {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      v[i] = {};
+      if (live && (inside(i) || dup[i] < V)) {
+        if (NV > 1 || FULL || C >= V) {
+          v[i] = Pack<T>::load(row + at[i]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < V; ++k)
+            if (k < C) v[i][k] = row[k];
+        }
+      }
+    }
+  }
+  __device__ __forceinline__ void store(T* row, int i, typename Pack<T>::Vec v) const {
+    if (!inside(i) && dup[i] >= V) return;
+    if (NV > 1 || FULL || C >= V) {
+      Pack<T>::store(row + at[i], v);
+    } else {
+#pragma unroll
+      for (int k = 0; k < V; ++k)
+        if (k < C) row[k] = v[k];
+    }
+  }
+  // a weight or bias row (NULL: `other`)
+  __device__ __forceinline__ void load_weight(const void* p, int type, int64_t row, float other, float (&w)[NV * V]) const {
+#pragma unroll
+    for (int k = 0; k < NV * V; ++k) w[k] = other;
+    if (!p) return;
+    if (type == MGNN_F32) {
+      const float* f = static_cast<const float*>(p) + row * C;
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        if (!inside(i) && dup[i] >= V) continue;
+        if (NV > 1 || FULL || C >= V) {
+#pragma unroll
+          for (int j = 0; j < V; j += 4) {
+            const auto q = Pack<float>::load(f + at[i] + j);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[i * V + j + k] = q[k];
+          }
+        } else {
+#pragma unroll
+          for (int k = 0; k < V; ++k)
+            if (k < C) w[i * V + k] = f[k];
+        }
+      }
+    } else {      // x's own 16-bit type
+      typename Pack<T>::Vec v[NV];
+      load(static_cast<const T*>(p) + row * C, true, v);
+#pragma unroll
+      for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int k = 0; k < V; ++k) w[i * V + k] = (float)v[i][k];
+    }
+  }
+};
+
+// Mean and sum of squared deviations of a row in the registers of TPR threads: two passes over the registers, so no digits
+// cancel.  n, inv_n: the wave's elements of the row.  Rows over several waves: each wave's own mean m_w and deviations M_w,
+// combined as M = sum of M_w + n_w (m_w - m)^2, which takes one barrier instead of two.
+template <typename T, int TPR, int NV, bool FULL>
+__device__ __forceinline__ void row_stats(const float (&v)[NV * Pack<T>::V], const Cols<T, TPR, NV, FULL>& cols, float n, float inv_n,
+                                          float inv_c, float4 (*red)[Shape<TPR>::WAVES], int parity, float& mean, float& m2) {
+  constexpr int V = Pack<T>::V, L = Shape<TPR>::L;
   float s = 0.f;
 #pragma unroll
-  for (int k = 0; k < NE; ++k) s += v[k];
+  for (int k = 0; k < NV * V; ++k) s += cols.counts(k / V, k % V) ? v[k] : 0.f;
   s = lanes_sum<L>(s);
-  int n = 0;      // this wave's elements of the row
-#pragma unroll
-  for (int i = 0; i < NE / V; ++i) {
-    const int first = ((TPR <= kWave ? 0 : (lane & ~(kWave - 1))) + i * TPR) * V;
-    n += min(max(C - first, 0), L * V);
-  }
-  mean = n > 0 ? s / (float)n : 0.f;
+  mean = s * inv_n;
   float q = 0.f;
 #pragma unroll
-  for (int k = 0; k < NE; ++k) {
-    const int col = (lane + (k / V) * TPR) * V + k % V;
-    const float d = v[k] - mean;
-    q += col < C ? d * d : 0.f;
+  for (int k = 0; k < NV * V; ++k) {
+    const float d = cols.counts(k / V, k % V) ? v[k] - mean : 0.f;
+    q = __builtin_fmaf(d, d, q);
   }
   m2 = lanes_sum<L>(q);
   if constexpr (TPR > kWave) {
     constexpr int W = Shape<TPR>::ROW_WAVES;
-    const int wave = threadIdx.x / kWave, first = wave / W * W;
-    if (threadIdx.x % kWave == 0) red[parity][wave] = make_float2(mean, m2);
+    const int wave = threadIdx.x / kWave;
+    if (threadIdx.x % kWave == 0) red[parity][wave] = make_float4(s, mean, m2, n);
     __syncthreads();
-    float total = 0.f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      int nw = 0;
-#pragma unroll
-      for (int i = 0; i < NE / V; ++i) nw += min(max(C - (w * kWave + i * TPR) * V, 0), kWave * V);
-      total += red[parity][first + w].x * (float)nw;
-    }
-    mean = total / (float)C;
-    m2 = 0.f;
-#pragma unroll
-    for (int w = 0; w < W; ++w) {
-      int nw = 0;
-#pragma unroll
-      for (int i = 0; i < NE / V; ++i) nw += min(max(C - (w * kWave + i * TPR) * V, 0), kWave * V);
-      const float2 r = red[parity][first + w];
-      const float d = r.x - mean;
-      m2 += nw > 0 ? r.y + (float)nw * (d * d) : 0.f;
-    }
+    const float4 r = red[parity][wave / W * W + threadIdx.x % W];      // each lane one wave's, then a sum over lanes
+    mean = lanes_sum<W>(r.x) * inv_c;
+    const float d = r.y - mean;
+    m2 = lanes_sum<W>(r.w > 0.f ? __builtin_fmaf(r.w * d, d, r.z) : 0.f);
   }
 }
 
-template <typename T, int TPR, int NV>
+template <typename T, int TPR, int NV, bool FULL>
 __global__ __launch_bounds__(Shape<TPR>::BLOCK) void ln_fwd_kernel(const T* x, int64_t ld, const void* weight, const void* bias,
                                                                    int wtype, T* y, float2* stats, int64_t rows, int C, float eps) {
-  constexpr int V = Pack<T>::V, NE = NV * V, SLOTS = Shape<TPR>::SLOTS;
-  __shared__ float2 red[2][Shape<TPR>::WAVES];
+  constexpr int V = Pack<T>::V, NE = NV * V, SLOTS = Shape<TPR>::SLOTS, L = Shape<TPR>::L;
+  __shared__ float4 red[2][Shape<TPR>::WAVES];
   const int lane = threadIdx.x % TPR, slot = threadIdx.x / TPR;
-  const int64_t g = blockIdx.y;
+  const int64_t g = blockIdx.y, step = (int64_t)gridDim.x * SLOTS;
+  const Cols<T, TPR, NV, FULL> cols(lane, C);
+  const float n = lanes_sum<L>((float)cols.count()), inv_n = n > 0.f ? 1.f / n : 0.f, inv_c = 1.f / (float)C;
+  x += g * rows * ld;
+  y += g * rows * C;
+  int64_t base = (int64_t)blockIdx.x * SLOTS, row = base + slot;
+  typename Pack<T>::Vec next[NV];
+  cols.load(x + row * ld, row < rows, next);
   float w[NE], b[NE];
-#pragma unroll
-  for (int k = 0; k < NE; ++k) {
-    const int col = (lane + (k / V) * TPR) * V + k % V;
-    w[k] = weight && col < C ? load_as_float(weight, wtype, g * C + col) : 1.f;
-    b[k] = bias && col < C ? load_as_float(bias, wtype, g * C + col) : 0.f;
-  }
+  cols.load_weight(weight, wtype, g, 1.f, w);
+  cols.load_weight(bias, wtype, g, 0.f, b);
   int parity = 0;
-  for (int64_t base = (int64_t)blockIdx.x * SLOTS; base < rows; base += (int64_t)gridDim.x * SLOTS, parity ^= 1) {
-    const int64_t row = g * rows + base + slot;
-    const bool live = base + slot < rows;
+  for (; base < rows; base += step, row += step, parity ^= 1) {
     float v[NE];
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int col = (lane + i * TPR) * V;
-      typename Pack<T>::Vec p = {};
-      if (live && col < C) p = load_part(x + row * ld, col, C);
-#pragma unroll
-      for (int k = 0; k < V; ++k) v[i * V + k] = (float)p[k];
-    }
+    for (int k = 0; k < NE; ++k) v[k] = (float)next[k / V][k % V];
+    cols.load(x + (row + step) * ld, row + step < rows, next);      // under the sums of this row
     float mean, m2;
-    row_stats<TPR, NE, V>(v, lane, C, red, parity, mean, m2);
-    const float rstd = 1.f / sqrtf(m2 / (float)C + eps);
-    if (live) {
-      if (stats && lane == 0) stats[row] = make_float2(mean, rstd);
+    row_stats<T, TPR, NV, FULL>(v, cols, n, inv_n, inv_c, red, parity, mean, m2);
+    const float rstd = rsqrtf(__builtin_fmaf(m2, inv_c, eps));
+    if (row < rows) {
+      if (stats && lane == 0) stats[g * rows + row] = make_float2(mean, rstd);
 #pragma unroll
       for (int i = 0; i < NV; ++i) {
-        const int col = (lane + i * TPR) * V;
         typename Pack<T>::Vec p;
 #pragma unroll
         for (int k = 0; k < V; ++k) p[k] = (T)__builtin_fmaf((v[i * V + k] - mean) * rstd, w[i * V + k], b[i * V + k]);
-        if (col < C) store_part(y + row * C, col, C, p);
+        cols.store(y + row * C, i, p);
       }
     }
   }
@@ -208,101 +279,107 @@ __device__ __forceinline__ void slots_sum(float (&acc)[NE], float* lds) {
 
 // partial: [groups][blocks][2][C] floats (this workgroup's shares of dweight and dbias), or NULL with one block per group:
 // then dweight / dbias are written here
-template <typename T, int TPR, int NV>
+template <typename T, int TPR, int NV, bool FULL>
 __global__ __launch_bounds__(Shape<TPR>::BLOCK) void ln_bwd_kernel(const T* x, int64_t ld, const T* dy, const void* weight,
                                                                    int wtype, const float2* stats, T* dx, float* partial,
                                                                    void* dweight, void* dbias, int64_t rows, int C) {
-  constexpr int V = Pack<T>::V, NE = NV * V, SLOTS = Shape<TPR>::SLOTS, WAVES = Shape<TPR>::WAVES;
-  constexpr int L = TPR < kWave ? TPR : kWave;
+  constexpr int V = Pack<T>::V, NE = NV * V, SLOTS = Shape<TPR>::SLOTS, WAVES = Shape<TPR>::WAVES, L = Shape<TPR>::L;
   constexpr int SETS = TPR < kWave ? WAVES : SLOTS, WIDTH = TPR < kWave ? kWave : TPR;
+  // 16 elements a thread in workgroups of 1024: the running sums take 128 KB of LDS, so that the next row fits the registers
+  constexpr bool SUMS_IN_LDS = TPR == 1024 && NE >= 16;
   __shared__ float2 red[2][WAVES];
-  __shared__ float fold[SETS > 1 ? SETS / 2 * NE * WIDTH : 1];
+  __shared__ float fold[SUMS_IN_LDS ? 2 * NE * TPR : SETS > 1 ? SETS / 2 * NE * WIDTH : 1];
   const int lane = threadIdx.x % TPR, slot = threadIdx.x / TPR;
-  const int64_t g = blockIdx.y;
+  const int64_t g = blockIdx.y, step = (int64_t)gridDim.x * SLOTS;
+  const Cols<T, TPR, NV, FULL> cols(lane, C);
   const float inv_c = 1.f / (float)C;
+  x += g * rows * ld;
+  dy += g * rows * C;
+  stats += g * rows;
+  int64_t base = (int64_t)blockIdx.x * SLOTS, row = base + slot;
+  typename Pack<T>::Vec next_x[NV], next_d[NV];
+  float2 next_st = row < rows ? stats[row] : make_float2(0.f, 0.f);
+  cols.load(x + row * ld, row < rows, next_x);
+  cols.load(dy + row * C, row < rows, next_d);
   float w[NE], aw[NE], ab[NE];
+  cols.load_weight(weight, wtype, g, 1.f, w);
 #pragma unroll
   for (int k = 0; k < NE; ++k) {
-    const int col = (lane + (k / V) * TPR) * V + k % V;
-    w[k] = weight && col < C ? load_as_float(weight, wtype, g * C + col) : 1.f;
     aw[k] = ab[k] = 0.f;
+    if constexpr (SUMS_IN_LDS) fold[k * TPR + lane] = fold[(NE + k) * TPR + lane] = 0.f;
   }
   int parity = 0;
-  for (int64_t base = (int64_t)blockIdx.x * SLOTS; base < rows; base += (int64_t)gridDim.x * SLOTS, parity ^= 1) {
-    const int64_t row = g * rows + base + slot;
-    const bool live = base + slot < rows;
-    const float2 st = live ? stats[row] : make_float2(0.f, 0.f);
+  for (; base < rows; base += step, row += step, parity ^= 1) {
+    const float2 st = next_st;
     float h[NE], e[NE];
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int col = (lane + i * TPR) * V;
-      typename Pack<T>::Vec px = {}, pd = {};
-      if (live && col < C) {
-        px = load_part(x + row * ld, col, C);
-        pd = load_part(dy + row * C, col, C);
-      }
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const int j = i * V + k;
-        const float d = (float)pd[k];
-        h[j] = ((float)px[k] - st.x) * st.y;
-        if (col + k >= C) h[j] = 0.f;      // past the end x is 0, which is no element of the row
-        e[j] = d * w[j];
-        s1 += e[j];
-        s2 = __builtin_fmaf(e[j], h[j], s2);
+    for (int j = 0; j < NE; ++j) {
+      const float d = (float)next_d[j / V][j % V];      // 0 past the row's end and past the last row
+      h[j] = ((float)next_x[j / V][j % V] - st.x) * st.y;
+      e[j] = d * w[j];
+      s1 += cols.counts(j / V, j % V) ? e[j] : 0.f;
+      s2 += cols.counts(j / V, j % V) ? e[j] * h[j] : 0.f;
+      if constexpr (SUMS_IN_LDS) {
+        fold[j * TPR + lane] = __builtin_fmaf(d, h[j], fold[j * TPR + lane]);
+        fold[(NE + j) * TPR + lane] += d;
+      } else {
         aw[j] = __builtin_fmaf(d, h[j], aw[j]);
         ab[j] += d;
       }
     }
+    const bool more = row + step < rows;
+    next_st = more ? stats[row + step] : make_float2(0.f, 0.f);
+    cols.load(x + (row + step) * ld, more, next_x);
+    cols.load(dy + (row + step) * C, more, next_d);
     if (dx) {
       s1 = lanes_sum<L>(s1);
       s2 = lanes_sum<L>(s2);
       if constexpr (TPR > kWave) {
         constexpr int W = Shape<TPR>::ROW_WAVES;
-        const int wave = threadIdx.x / kWave, first = wave / W * W;
+        const int wave = threadIdx.x / kWave;
         if (threadIdx.x % kWave == 0) red[parity][wave] = make_float2(s1, s2);
         __syncthreads();
-        s1 = s2 = 0.f;
-#pragma unroll
-        for (int k = 0; k < W; ++k) {
-          const float2 r = red[parity][first + k];
-          s1 += r.x;
-          s2 += r.y;
-        }
+        const float2 r = red[parity][wave / W * W + threadIdx.x % W];
+        s1 = lanes_sum<W>(r.x);
+        s2 = lanes_sum<W>(r.y);
       }
       s1 *= inv_c;
       s2 *= inv_c;
-      if (live) {
+      if (row < rows) {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-          const int col = (lane + i * TPR) * V;
           typename Pack<T>::Vec p;
 #pragma unroll
           for (int k = 0; k < V; ++k) {
             const int j = i * V + k;
             p[k] = (T)(st.y * (e[j] - __builtin_fmaf(h[j], s2, s1)));
           }
-          if (col < C) store_part(dx + row * C, col, C, p);
+          cols.store(dx + (g * rows + row) * C, i, p);
         }
       }
     }
   }
   if (!dweight && !dbias) return;
-  slots_sum<TPR, NE>(aw, fold);
-  slots_sum<TPR, NE>(ab, fold);
+  if constexpr (SUMS_IN_LDS) {
+#pragma unroll
+    for (int k = 0; k < NE; ++k) aw[k] = fold[k * TPR + lane], ab[k] = fold[(NE + k) * TPR + lane];
+  } else {
+    slots_sum<TPR, NE>(aw, fold);
+    slots_sum<TPR, NE>(ab, fold);
+  }
   if (threadIdx.x >= TPR) return;
   float* share = partial ? partial + (g * gridDim.x + blockIdx.x) * 2 * C : nullptr;
 #pragma unroll
-  for (int k = 0; k < NE; ++k) {
-    const int col = (lane + (k / V) * TPR) * V + k % V;
-    if (col >= C) continue;
+  for (int j = 0; j < NE; ++j) {
+    if (!cols.counts(j / V, j % V)) continue;
+    const int col = cols.at[j / V] + j % V;
     if (share) {
-      share[col] = aw[k];
-      share[C + col] = ab[k];
+      share[col] = aw[j];
+      share[C + col] = ab[j];
     } else {
-      if (dweight) store_from_float(dweight, wtype, g * C + col, aw[k]);
-      if (dbias) store_from_float(dbias, wtype, g * C + col, ab[k]);
+      if (dweight) store_from_float(dweight, wtype, g * C + col, aw[j]);
+      if (dbias) store_from_float(dbias, wtype, g * C + col, ab[j]);
     }
   }
 }
@@ -336,26 +413,48 @@ int launched() { return hipGetLastError() == hipSuccess ? MGNN_OK : MGNN_ERR_LAU
 
 int elem_bytes(int type) { return type == MGNN_F32 ? 4 : type == MGNN_BF16 || type == MGNN_F16 ? 2 : 0; }
 
-// threads per row (a power of two) and vectors per thread of a row of C elements
+// Threads per row (a power of two) and vectors per thread of a row of C elements.  Rows that fit 64 vectors: one per lane,
+// the fewest lanes.  Longer ones: two per thread, which beat one (half the waves meet at the barrier) and four (registers)
+// in the backward pass and lose nothing in the forward one: bf16 4096 columns x 16384 rows, 256 x 2 / 512 x 1 / 128 x 4:
+// forward 50.3 / 50.4 / 49.0 us, backward 83 / 85 / 94; fp32 1024 columns, 128 x 2 / 256 x 1 / 64 x 4: backward 41.4 / 44.8 / 41.6.
 struct RowSplit {
   int tpr, nv;
 };
 RowSplit row_split(int C, int type) {
   const int V = 16 / elem_bytes(type), vecs = (C + V - 1) / V;
+  const int nv = vecs <= kWave ? 1 : vecs <= 2048 ? 2 : 4;
   int tpr = 1;
-  while (tpr < vecs && tpr < 1024) tpr <<= 1;
-  int nv = 1;
-  while (tpr * nv < vecs) nv <<= 1;
+  while (tpr * nv < vecs) tpr <<= 1;
   return {tpr, nv};
 }
-int slots_of(const RowSplit& s) { return s.tpr > 256 ? 1 : 256 / s.tpr; }
+int block_of(const RowSplit& s) { return s.tpr > 256 ? s.tpr : 256; }
 
-// workgroups per group of the backward pass: each leaves one row of shares to be added up
+// Workgroups per group for `want` workgroup-steps of rows each, at most about `most` workgroups in all groups: every one
+// takes the same number of steps, the last one apart.
+int64_t even_blocks(int64_t want, int64_t groups, int64_t most) {
+  const int64_t cap = std::max<int64_t>(1, most / groups), steps = (want + cap - 1) / cap;
+  return steps ? (want + steps - 1) / steps : 1;
+}
+
+// Forward: workgroups stay, keep their weight rows in registers and load the next row under the sums of this one.  16 waves
+// per CU carry fp32 rows (3 x 409600 rows of 128: 229 us, 8 waves 294, 32 waves 249) and rows over several waves; 16-bit
+// rows within a wave have twice the arithmetic per byte and want 32 (3 x 409600 of 64: 62 us, 16 waves 72).  Work that does
+// not fill the card once over goes out one step per workgroup.
+int64_t forward_blocks(int64_t groups, int64_t rows, int C, int type) {
+  const RowSplit s = row_split(C, type);
+  const int64_t slots = block_of(s) / s.tpr, want = (rows + slots - 1) / slots;
+  const int64_t full = 2048 * 256 / block_of(s), most = type != MGNN_F32 && s.tpr <= kWave ? full : full / 2;
+  return want * groups <= full ? want : even_blocks(want, groups, most);
+}
+
+// Backward: each workgroup leaves one row of shares of dweight and dbias to be added up, so fewer are better as long as
+// two of up to 512 threads stand on every CU (bf16 16384 x 4096, 256 / 512 / 1024 / 2048 workgroups: 106 / 83 / 104 / 115
+// us; fp32 3 x 409600 x 128: 525 / 355 / 369 / 383); and at least four steps each.
 int64_t backward_blocks(int64_t groups, int64_t rows, int C, int type) {
   const RowSplit s = row_split(C, type);
-  const int64_t slots = slots_of(s), want = (rows + 4 * slots - 1) / (4 * slots);
-  const int64_t cap = std::max<int64_t>(1, (s.tpr > 256 ? 262144 / s.tpr : 1024) / groups);
-  return std::max<int64_t>(1, std::min(want, cap));
+  const int64_t slots = block_of(s) / s.tpr, want = (rows + slots - 1) / slots;
+  const int64_t most = s.tpr > 512 ? 256 : 512;
+  return std::max<int64_t>(1, std::min((want + 3) / 4, even_blocks(want, groups, most)));
 }
 
 int check_ln(int64_t ld, int64_t groups, int64_t rows, int C, int type, int wtype) {
@@ -366,35 +465,35 @@ int check_ln(int64_t ld, int64_t groups, int64_t rows, int C, int type, int wtyp
   return MGNN_OK;
 }
 
-// calls f.template operator()<TPR, NV>() for the split
-template <typename F>
-void with_split(const RowSplit& s, F f) {
+// calls f.template operator()<TPR, NV, FULL>() for the split of rows of C elements
+template <typename T, typename F>
+void with_split(const RowSplit& s, int C, F f) {
+  const bool full = C == s.tpr * s.nv * Pack<T>::V;
   switch (s.tpr * 8 + s.nv) {
-    case 1 * 8 + 1: return f.template operator()<1, 1>();
-    case 2 * 8 + 1: return f.template operator()<2, 1>();
-    case 4 * 8 + 1: return f.template operator()<4, 1>();
-    case 8 * 8 + 1: return f.template operator()<8, 1>();
-    case 16 * 8 + 1: return f.template operator()<16, 1>();
-    case 32 * 8 + 1: return f.template operator()<32, 1>();
-    case 64 * 8 + 1: return f.template operator()<64, 1>();
-    case 128 * 8 + 1: return f.template operator()<128, 1>();
-    case 256 * 8 + 1: return f.template operator()<256, 1>();
-    case 512 * 8 + 1: return f.template operator()<512, 1>();
-    case 1024 * 8 + 1: return f.template operator()<1024, 1>();
-    case 1024 * 8 + 2: return f.template operator()<1024, 2>();
-    case 1024 * 8 + 4: return f.template operator()<1024, 4>();
+    case 1 * 8 + 1: return full ? f.template operator()<1, 1, true>() : f.template operator()<1, 1, false>();
+    case 2 * 8 + 1: return full ? f.template operator()<2, 1, true>() : f.template operator()<2, 1, false>();
+    case 4 * 8 + 1: return full ? f.template operator()<4, 1, true>() : f.template operator()<4, 1, false>();
+    case 8 * 8 + 1: return full ? f.template operator()<8, 1, true>() : f.template operator()<8, 1, false>();
+    case 16 * 8 + 1: return full ? f.template operator()<16, 1, true>() : f.template operator()<16, 1, false>();
+    case 32 * 8 + 1: return full ? f.template operator()<32, 1, true>() : f.template operator()<32, 1, false>();
+    case 64 * 8 + 1: return full ? f.template operator()<64, 1, true>() : f.template operator()<64, 1, false>();
+    case 64 * 8 + 2: return full ? f.template operator()<64, 2, true>() : f.template operator()<64, 2, false>();
+    case 128 * 8 + 2: return full ? f.template operator()<128, 2, true>() : f.template operator()<128, 2, false>();
+    case 256 * 8 + 2: return full ? f.template operator()<256, 2, true>() : f.template operator()<256, 2, false>();
+    case 512 * 8 + 2: return full ? f.template operator()<512, 2, true>() : f.template operator()<512, 2, false>();
+    case 1024 * 8 + 2: return full ? f.template operator()<1024, 2, true>() : f.template operator()<1024, 2, false>();
+    case 1024 * 8 + 4:      // fp32 rows of more than 8192
+      if constexpr (std::is_same_v<T, float>) return full ? f.template operator()<1024, 4, true>() : f.template operator()<1024, 4, false>();
   }
 }
 
 template <typename T>
 struct LnFwd {
-  const T* x; int64_t ld; const void *weight, *bias; int wtype; T* y; float2* stats; int64_t groups, rows; int C; float eps;
+  const T* x; int64_t ld; const void *weight, *bias; int wtype; T* y; float2* stats; int64_t groups, rows, blocks; int C; float eps;
   hipStream_t stream;
-  template <int TPR, int NV>
+  template <int TPR, int NV, bool FULL>
   void operator()() {
-    const int64_t slots = Shape<TPR>::SLOTS, want = (rows + slots - 1) / slots;
-    const int64_t cap = std::max<int64_t>(1, 16384 / groups);
-    hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, NV>), dim3((unsigned)std::min(want, cap), (unsigned)groups), dim3(Shape<TPR>::BLOCK), 0,
+    hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, NV, FULL>), dim3((unsigned)blocks, (unsigned)groups), dim3(Shape<TPR>::BLOCK), 0,
                        stream, x, ld, weight, bias, wtype, y, stats, rows, C, eps);
   }
 };
@@ -403,9 +502,9 @@ template <typename T>
 struct LnBwd {
   const T* x; int64_t ld; const T* dy; const void* weight; int wtype; const float2* stats; T* dx; float* partial;
   void *dweight, *dbias; int64_t groups, rows, blocks; int C; hipStream_t stream;
-  template <int TPR, int NV>
+  template <int TPR, int NV, bool FULL>
   void operator()() {
-    hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, NV>), dim3((unsigned)blocks, (unsigned)groups), dim3(Shape<TPR>::BLOCK), 0, stream, x,
+    hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, NV, FULL>), dim3((unsigned)blocks, (unsigned)groups), dim3(Shape<TPR>::BLOCK), 0, stream, x,
                        ld, dy, weight, wtype, stats, dx, partial, dweight, dbias, rows, C);
   }
 };
@@ -652,8 +751,8 @@ int mgnn_layer_norm(const void* x, int64_t ld, const void* weight, const void* b
   if (!x || !y) return MGNN_ERR_VALUE;
   auto go = [&](auto zero) {
     using T = decltype(zero);
-    with_split(row_split(C, type), LnFwd<T>{static_cast<const T*>(x), ld, weight, bias, wtype, static_cast<T*>(y), reinterpret_cast<float2*>(stats),
-                                            groups, rows, C, (float)eps, (hipStream_t)stream});
+    with_split<T>(row_split(C, type), C, LnFwd<T>{static_cast<const T*>(x), ld, weight, bias, wtype, static_cast<T*>(y), reinterpret_cast<float2*>(stats),
+                                            groups, rows, forward_blocks(groups, rows, C, type), C, (float)eps, (hipStream_t)stream});
   };
   if (type == MGNN_F32) go(0.f);
   else if (type == MGNN_BF16) go((__bf16)0.f);
@@ -682,7 +781,7 @@ int mgnn_layer_norm_backward(const void* x, int64_t ld, const void* dy, const vo
   float* partial = join ? static_cast<float*>(workspace) : nullptr;
   auto go = [&](auto zero) {
     using T = decltype(zero);
-    with_split(row_split(C, type), LnBwd<T>{static_cast<const T*>(x), ld, static_cast<const T*>(dy), weight, wtype,
+    with_split<T>(row_split(C, type), C, LnBwd<T>{static_cast<const T*>(x), ld, static_cast<const T*>(dy), weight, wtype,
                                             reinterpret_cast<const float2*>(stats), static_cast<T*>(dx), partial, dweight, dbias, groups,
                                             rows, blocks, C, (hipStream_t)stream});
   };
