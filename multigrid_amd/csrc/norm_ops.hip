@@ -56,25 +56,39 @@ __device__ __forceinline__ void store_from_float(void* p, int type, int64_t i, f
 }
 
 // Sum over aligned groups of L lanes, in every lane of the group (all 64 lanes take part), on the vector units alone: lane
-// permutations within 16 lanes, then whole rows of 16 and halves of the wave swapped between two registers.
-template <int CTRL>
-__device__ __forceinline__ float dpp_add(float v) {
-  return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+// permutations within 16 lanes, then whole rows of 16 and halves of the wave swapped between two registers.  float or double.
+template <int CTRL, typename F>
+__device__ __forceinline__ F dpp_add(F v) {
+  if constexpr (sizeof(F) == 4) {
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+  } else {
+    const int lo = __builtin_amdgcn_update_dpp(0, __double2loint(v), CTRL, 0xf, 0xf, true);
+    const int hi = __builtin_amdgcn_update_dpp(0, __double2hiint(v), CTRL, 0xf, 0xf, true);
+    return v + __hiloint2double(hi, lo);
+  }
 }
-template <int L>
-__device__ __forceinline__ float lanes_sum(float v) {
+template <bool HALVES, typename F>      // + the other half of the wave, or the other 16 lanes of a half
+__device__ __forceinline__ F swap_add(F v) {
+  auto both = [](unsigned u) {
+    if constexpr (HALVES) return __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    else return __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  };
+  if constexpr (sizeof(F) == 4) {
+    const auto r = both(__float_as_uint(v));
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+  } else {
+    const auto lo = both((unsigned)__double2loint(v)), hi = both((unsigned)__double2hiint(v));
+    return __hiloint2double((int)hi[0], (int)lo[0]) + __hiloint2double((int)hi[1], (int)lo[1]);
+  }
+}
+template <int L, typename F>
+__device__ __forceinline__ F lanes_sum(F v) {
   if constexpr (L >= 2) v = dpp_add<0xB1>(v);       // lane ^ 1
   if constexpr (L >= 4) v = dpp_add<0x4E>(v);       // lane ^ 2
   if constexpr (L >= 8) v = dpp_add<0x141>(v);      // mirrored within 8: the other four lanes
   if constexpr (L >= 16) v = dpp_add<0x140>(v);     // mirrored within 16: the other eight
-  if constexpr (L >= 32) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  }
-  if constexpr (L >= 64) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
-  }
+  if constexpr (L >= 32) v = swap_add<false>(v);
+  if constexpr (L >= 64) v = swap_add<true>(v);
   return v;
 }
 
@@ -526,16 +540,12 @@ struct GradTable {
 };
 static_assert(sizeof(GradTable) <= 3800, "kernel arguments hold 4 KB");
 
-__device__ __forceinline__ double block_sum(double v, double* lds) {      // in every thread
-#pragma unroll
-  for (int s = 1; s < kWave; s <<= 1) v += __shfl_xor(v, s);
+template <int BLOCK>
+__device__ __forceinline__ double block_sum(double v, double* lds) {      // in every thread of the first wave
+  v = lanes_sum<kWave>(v);
   if (threadIdx.x % kWave == 0) lds[threadIdx.x / kWave] = v;
   __syncthreads();
-  double t = 0.0;
-#pragma unroll
-  for (int k = 0; k < kBlock / kWave; ++k) t += lds[k];
-  __syncthreads();
-  return t;
+  return threadIdx.x < kWave ? lanes_sum<BLOCK / kWave>(lds[threadIdx.x % (BLOCK / kWave)]) : 0.0;
 }
 
 __device__ __forceinline__ int find_tensor(const GradTable& t, int chunk) {
@@ -577,20 +587,26 @@ __global__ __launch_bounds__(kBlock) void grad_squares_kernel(GradTable t, doubl
     else if (t.type[i] == MGNN_BF16) acc += chunk_squares(static_cast<const __bf16*>(t.src[i]) + off, n);
     else acc += chunk_squares(static_cast<const _Float16*>(t.src[i]) + off, n);
   }
-  acc = block_sum(acc, lds);
+  acc = block_sum<kBlock>(acc, lds);
   if (threadIdx.x == 0) partial[g * rows_of_group + row + blockIdx.x] = acc;
 }
 
+// Group g's norm from the partial sums, in every thread of the first wave
 __device__ __forceinline__ double group_norm(const double* partial, int64_t g, int rows_of_group, double* lds) {
   double acc = 0.0;
   for (int k = threadIdx.x; k < rows_of_group; k += kBlock) acc += partial[g * rows_of_group + k];
-  return sqrt(block_sum(acc, lds));
+  const double sum = block_sum<kBlock>(acc, lds);
+  return threadIdx.x < kWave ? sqrt(sum) : 0.0;
 }
 
-// min(1, max_norm / (norm + 1e-6)); NaN stays NaN
-__device__ __forceinline__ float clip_factor(double norm, double max_norm) {
-  const float f = (float)(max_norm / (norm + 1e-6));
-  return f > 1.f ? 1.f : f;
+// min(1, max_norm / (norm + 1e-6)), where NaN stays NaN; norm is the first wave's, which alone does the fp64 division
+__device__ __forceinline__ float clip_factor(double norm, double max_norm, float* lds) {
+  if (threadIdx.x < kWave) {
+    const float f = (float)(max_norm / (norm + 1e-6));
+    if (threadIdx.x == 0) *lds = f > 1.f ? 1.f : f;
+  }
+  __syncthreads();
+  return *lds;
 }
 
 __global__ __launch_bounds__(kBlock) void grad_norm_kernel(const double* partial, int rows_of_group, float* norms) {
@@ -617,12 +633,13 @@ __device__ __forceinline__ void chunk_scale(const T* p, T* q, int64_t n, float f
 __global__ __launch_bounds__(kBlock) void grad_scale_kernel(GradTable t, const double* partial, int rows_of_group, double max_norm,
                                                             float* norms) {
   __shared__ double lds[kBlock / kWave];
+  __shared__ float factor;
   const int64_t g = blockIdx.y;
   const double norm = group_norm(partial, g, rows_of_group, lds);
-  const float f = clip_factor(norm, max_norm);
+  const float f = clip_factor(norm, max_norm, &factor);
   if (norms && blockIdx.x == 0 && threadIdx.x == 0) norms[g] = (float)norm;
-  const int chunks = t.end[t.count - 1];
-  for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
+  // from the end on, which was read last: what the caches still hold of it is not read from memory again
+  for (int c = t.end[t.count - 1] - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {
     const int i = find_tensor(t, c);
     if (f == 1.f && t.src[i] == t.dst[i]) continue;      // a factor of 1 in place: nothing changes
     const int64_t at = (int64_t)(c - (i ? t.end[i - 1] : 0)) * (kChunkBytes / (t.type[i] == MGNN_F32 ? 4 : 2));
@@ -630,6 +647,134 @@ __global__ __launch_bounds__(kBlock) void grad_scale_kernel(GradTable t, const d
     if (t.type[i] == MGNN_F32) chunk_scale(static_cast<const float*>(t.src[i]) + off, static_cast<float*>(t.dst[i]) + off, n, f);
     else if (t.type[i] == MGNN_BF16) chunk_scale(static_cast<const __bf16*>(t.src[i]) + off, static_cast<__bf16*>(t.dst[i]) + off, n, f);
     else chunk_scale(static_cast<const _Float16*>(t.src[i]) + off, static_cast<_Float16*>(t.dst[i]) + off, n, f);
+  }
+}
+
+// Norms and clipping of gradients that one workgroup per group holds in its registers, SLOTS vectors of 16 bytes a thread:
+// one launch, and every element is read once.  The list's vectors are numbered through (t.end: vectors up to and with a
+// tensor); a tensor's last vector ends at its end and overlaps the one before, which counts the common elements; both
+// write the same values.  FLOATS: all of the list is fp32.  max_norm < 0: the norms alone.
+constexpr int kSmallBlock = 1024;
+constexpr int kSearch = 64;          // the largest power of two up to kTensors
+static_assert(kSearch <= kTensors && kTensors < 2 * kSearch && kTensors <= kSmallBlock);
+constexpr int kSmallSlots = 16;      // at most: 64 of the 128 registers a thread of 1024 has
+template <typename T>
+__device__ __forceinline__ double raw_squares(uint4 raw, int skip, int n) {      // elements skip .. n-1 of the vector
+  constexpr int V = Pack<T>::V;
+  typename Pack<T>::Vec v = __builtin_bit_cast(typename Pack<T>::Vec, raw);
+  if (skip > 0 || n < V) {      // a tensor's last vector
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = k >= skip && k < n ? v[k] : (T)0.f;
+  }
+  double acc = 0.0;
+#pragma unroll
+  for (int k = 0; k < V; ++k) acc = __builtin_fma((double)(float)v[k], (double)(float)v[k], acc);
+  return acc;
+}
+template <typename T>
+__device__ __forceinline__ uint4 raw_load(const T* p, int n) {
+  constexpr int V = Pack<T>::V;
+  typename Pack<T>::Vec v = {};
+  if (n >= V) {
+    v = Pack<T>::load(p);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (k < n) v[k] = p[k];
+  }
+  return __builtin_bit_cast(uint4, v);
+}
+template <typename T>
+__device__ __forceinline__ void raw_scale(T* p, uint4 raw, int n, float f) {
+  constexpr int V = Pack<T>::V;
+  typename Pack<T>::Vec v = __builtin_bit_cast(typename Pack<T>::Vec, raw);
+#pragma unroll
+  for (int k = 0; k < V; ++k) v[k] = (T)((float)v[k] * f);
+  if (n >= V) {
+    Pack<T>::store(p, v);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k)
+      if (k < n) p[k] = v[k];
+  }
+}
+
+template <int SLOTS, bool FLOATS>
+__global__ __launch_bounds__(kSmallBlock) void grad_small_kernel(GradTable t, double max_norm, float* norms) {
+  __shared__ double lds[kSmallBlock / kWave];
+  __shared__ int32_t end[2 * kSearch - 1];
+  __shared__ const char* from[kTensors];
+  __shared__ char* to[kTensors];
+  __shared__ int32_t len[kTensors];
+  __shared__ uint8_t type[kTensors], first[SLOTS * kSmallBlock / kWave];
+  __shared__ float factor;
+  const auto type_of = [&](int i) { return FLOATS ? MGNN_F32 : (int)type[i]; };
+  const int64_t g = blockIdx.x;
+  if (threadIdx.x >= t.count && threadIdx.x < 2 * kSearch - 1) end[threadIdx.x] = INT32_MAX;
+  if (threadIdx.x < t.count) {
+    const int i = threadIdx.x;
+    const int64_t off = g * t.n[i] * (t.type[i] == MGNN_F32 ? 4 : 2);
+    end[i] = t.end[i];
+    from[i] = static_cast<const char*>(t.src[i]) + off;
+    to[i] = t.dst[i] ? static_cast<char*>(t.dst[i]) + off : nullptr;
+    len[i] = (int32_t)t.n[i];
+    type[i] = t.type[i];
+  }
+  __syncthreads();
+  const int vectors = end[t.count - 1];
+  // the tensor of every wave's first vector: the number of tensors that end at or before it
+  if (threadIdx.x < SLOTS * kSmallBlock / kWave) {
+    int i = 0;
+    for (int half = kSearch; half >= 1; half >>= 1)      // i + half <= 2 * kSearch - 1, the list's last entry
+      if (half <= t.count && end[i + half - 1] <= (int)threadIdx.x * kWave) i += half;
+    first[threadIdx.x] = (uint8_t)i;
+  }
+  __syncthreads();
+  int which[SLOTS], stop[SLOTS];
+#pragma unroll
+  for (int k = 0; k < SLOTS; ++k) which[k] = first[k * (kSmallBlock / kWave) + threadIdx.x / kWave];
+#pragma unroll
+  for (int k = 0; k < SLOTS; ++k) stop[k] = end[which[k]];
+#pragma unroll
+  for (int k = 0; k < SLOTS; ++k)
+    while (k * kSmallBlock + (int)threadIdx.x >= stop[k]) stop[k] = end[++which[k]];      // ends at a padding entry at the latest
+  uint4 raw[SLOTS];
+  int place[SLOTS];      // tensor << 20 | first element; -1: no vector
+  static_assert(kSmallSlots * kSmallBlock * 8 <= 1 << 20 && kTensors < 1 << 11);
+  double acc = 0.0;
+#pragma unroll
+  for (int k = 0; k < SLOTS; ++k) {
+    const int v = k * kSmallBlock + threadIdx.x, i = which[k];
+    place[k] = -1;
+    if (v < vectors) {
+      const int V = type_of(i) == MGNN_F32 ? 4 : 8;
+      const int at = max(min((v - (i ? end[i - 1] : 0)) * V, len[i] - V), 0);
+      place[k] = i << 20 | at;
+      raw[k] = type_of(i) == MGNN_F32 ? raw_load(reinterpret_cast<const float*>(from[i]) + at, len[i])
+                                   : raw_load(reinterpret_cast<const _Float16*>(from[i]) + at, len[i]);
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < SLOTS; ++k) {
+    if (place[k] < 0) continue;
+    const int i = place[k] >> 20, ty = type_of(i), V = ty == MGNN_F32 ? 4 : 8;
+    const int skip = (k * kSmallBlock + (int)threadIdx.x - (i ? end[i - 1] : 0)) * V - (place[k] & 0xfffff);
+    acc += ty == MGNN_F32 ? raw_squares<float>(raw[k], skip, len[i])
+                          : ty == MGNN_BF16 ? raw_squares<__bf16>(raw[k], skip, len[i]) : raw_squares<_Float16>(raw[k], skip, len[i]);
+  }
+  const double sum = block_sum<kSmallBlock>(acc, lds);
+  const double norm = threadIdx.x < kWave ? sqrt(sum) : 0.0;
+  if (threadIdx.x == 0) norms[g] = (float)norm;
+  if (max_norm < 0.0) return;
+  const float f = clip_factor(norm, max_norm, &factor);
+#pragma unroll
+  for (int k = 0; k < SLOTS; ++k) {
+    if (place[k] < 0) continue;
+    const int i = place[k] >> 20, at = place[k] & 0xfffff, ty = type_of(i);
+    if (f == 1.f && from[i] == to[i]) continue;      // a factor of 1 in place: nothing changes
+    if (ty == MGNN_F32) raw_scale(reinterpret_cast<float*>(to[i]) + at, raw[k], len[i], f);
+    else if (ty == MGNN_BF16) raw_scale(reinterpret_cast<__bf16*>(to[i]) + at, raw[k], len[i], f);
+    else raw_scale(reinterpret_cast<_Float16*>(to[i]) + at, raw[k], len[i], f);
   }
 }
 
@@ -642,7 +787,8 @@ __global__ void zero_norms_kernel(float* norms, int groups) {
 struct GradPlan {
   std::vector<GradTable> tables;
   std::vector<int> blocks;
-  int rows = 0;      // partial sums per group
+  int rows = 0;      // partial sums per group; 0 with a table: one workgroup per group does it all
+  int slots = 0;     // then its vectors per thread
 };
 
 // chunks a tensor is cut into; -1: not a tensor that the list may hold
@@ -677,6 +823,23 @@ int grad_plan(const void* const* src, void* const* dst, const int64_t* n, const 
     t.n[t.count] = n[i];
     t.type[t.count] = (uint8_t)type[i];
     t.end[t.count++] = (int32_t)chunks;
+  }
+  if (plan.tables.size() == 1) {
+    GradTable& t = plan.tables[0];
+    int64_t vectors = 0;
+    for (int i = 0; i < t.count; ++i) {
+      const int V = t.type[i] == MGNN_F32 ? 4 : 8;
+      vectors += t.n[i] / V + (t.n[i] % V != 0);
+      if (vectors > kSmallSlots * kSmallBlock) break;
+    }
+    if (vectors <= kSmallSlots * kSmallBlock) {
+      for (int i = 0, v = 0; i < t.count; ++i) {
+        const int V = t.type[i] == MGNN_F32 ? 4 : 8;
+        t.end[i] = v += (int)((t.n[i] + V - 1) / V);
+      }
+      plan.slots = (int)((vectors + 4 * kSmallBlock - 1) / (4 * kSmallBlock)) * 4;
+      return MGNN_OK;
+    }
   }
   for (const GradTable& t : plan.tables) {
     const int64_t cap = std::max<int64_t>(1, 1024 / groups);
@@ -721,6 +884,18 @@ int clip(const void* const* src, void* const* dst, const int64_t* n, const int32
     return launched();
   }
   if (dst && overlaps(src, dst, n, type, count, groups)) return MGNN_ERR_OVERLAP;
+  if (plan.slots) {
+    const GradTable& t = plan.tables[0];
+    const bool floats = std::all_of(t.type, t.type + t.count, [](uint8_t ty) { return ty == MGNN_F32; });
+    const auto pick = [&](auto all) {
+      constexpr bool F = decltype(all)::value;
+      return plan.slots == 4 ? grad_small_kernel<4, F> : plan.slots == 8 ? grad_small_kernel<8, F>
+             : plan.slots == 12 ? grad_small_kernel<12, F> : grad_small_kernel<kSmallSlots, F>;
+    };
+    const auto kernel = floats ? pick(std::true_type()) : pick(std::false_type());
+    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kSmallBlock), 0, stream, t, dst ? max_norm : -1.0, norms);
+    return launched();
+  }
   if (!workspace || (uintptr_t)workspace % 8 || workspace_bytes < plan.rows * groups * (int64_t)sizeof(double)) return MGNN_ERR_WORKSPACE;
   double* partial = static_cast<double*>(workspace);
   int row = 0;
@@ -733,7 +908,7 @@ int clip(const void* const* src, void* const* dst, const int64_t* n, const int32
     hipLaunchKernelGGL(grad_norm_kernel, dim3((unsigned)groups), dim3(kBlock), 0, stream, partial, plan.rows, norms);
     return launched();
   }
-  for (size_t k = 0; k < plan.tables.size(); ++k)
+  for (size_t k = plan.tables.size(); k-- > 0;)
     hipLaunchKernelGGL(grad_scale_kernel, dim3(plan.blocks[k], (unsigned)groups), dim3(kBlock), 0, stream, plan.tables[k], partial,
                        plan.rows, max_norm, k == 0 ? norms : nullptr);
   return launched();

@@ -11,6 +11,7 @@ Nothing is kept between calls: workspaces come from torch's allocator, so every 
 """
 import array
 import ctypes as C
+import functools
 import math
 
 import torch
@@ -51,13 +52,16 @@ def load():
   return _LIB
 
 
-def _check(rc, what):
+def _call(fn, dev, *args):
+  """fn(*args, stream) on dev, whose current stream it enqueues on."""
+  stream = torch._C._cuda_getCurrentRawStream(dev.index)
+  if torch.cuda.current_device() == dev.index:
+    rc = fn(*args, stream)
+  else:
+    with torch.cuda.device(dev):
+      rc = fn(*args, stream)
   if rc != 0:
-    raise (RuntimeError if rc == 2 else ValueError)('%s: %s (MGNN error %d)' % (what, ERRORS.get(rc, 'unknown'), rc))
-
-
-def _stream(dev):
-  return torch.cuda.current_stream(dev).cuda_stream
+    raise (RuntimeError if rc == 2 else ValueError)('%s: %s (MGNN error %d)' % (fn.__name__, ERRORS.get(rc, 'unknown'), rc))
 
 
 # ---- layer norm ----
@@ -90,67 +94,75 @@ def _ln_args(x, weight, bias, eps):
   return groups
 
 
-def _rows(x):
-  """x as [rows, cols] with contiguous rows at one distance (a view where there is one), and that distance."""
-  cols = x.shape[-1]
-  n = x.numel() // cols
-  x2 = x.reshape(n, cols)
-  if (cols > 1 and x2.stride(1) != 1) or (n > 1 and x2.stride(0) < cols):
-    x2 = x2.contiguous()
-  return x2, x2.stride(0) if n > 1 else cols
+def _rows(x, cols):
+  """x with its rows contiguous and at one distance (x itself or a view of it where that holds), and that distance."""
+  if x.is_contiguous():
+    return x, cols
+  x = x.reshape(-1, cols)
+  if (cols > 1 and x.stride(1) != 1) or (x.shape[0] > 1 and x.stride(0) < cols):
+    return x.contiguous(), cols
+  return x, x.stride(0) if x.shape[0] > 1 else cols
 
 
-def _ptr(t):
-  return None if t is None else t.data_ptr()
+@functools.lru_cache(maxsize=1024)
+def _workspace(groups, rows, cols, kind):
+  return load().mgnn_layer_norm_workspace(groups, rows, cols, kind)
 
 
 def _ln_forward(x, weight, bias, eps, groups, want_stats):
+  """y, and what the backward pass takes of the call: x by rows, its row distance, the statistics, the weight, the sizes."""
+  cols = x.shape[-1]
+  n = x.numel() // cols
+  x2, ld = _rows(x, cols)
+  y = torch.empty_like(x) if x2 is x else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+  w = b = None
+  kind = wkind = TYPES[x.dtype]
+  if weight is not None:
+    w = weight.contiguous()
+    wkind = TYPES[w.dtype]
+  if bias is not None:
+    b = bias.contiguous()
+    wkind = TYPES[b.dtype]
+  stats = torch.empty(2 * n, dtype=torch.float32, device=x.device) if want_stats else None
+  sizes = (groups, n // groups if groups else 0, cols)
+  _call(load().mgnn_layer_norm, x.device, x2.data_ptr(), ld, w.data_ptr() if weight is not None else None,
+        b.data_ptr() if bias is not None else None, y.data_ptr(), stats.data_ptr() if want_stats else None, *sizes, eps, kind, wkind)
+  return y, x2, ld, stats, w, sizes, (kind, wkind)
+
+
+def _ln_backward(ctx, dy):
+  x, stats, w = ctx.saved_tensors
+  ld, sizes, kinds, affine = ctx.plan
+  want_x, want_w, want_b = ctx.needs_input_grad[:3]
   dev = x.device
-  x2, ld = _rows(x)
-  n, cols = x2.shape
-  weight = None if weight is None else weight.contiguous()
-  bias = None if bias is None else bias.contiguous()
-  wt = weight if weight is not None else bias
-  y = torch.empty(x.shape, dtype=x.dtype, device=dev)
-  stats = torch.empty((n, 2), dtype=torch.float32, device=dev) if want_stats else None
-  with torch.cuda.device(dev):
-    _check(load().mgnn_layer_norm(x2.data_ptr(), ld, _ptr(weight), _ptr(bias), y.data_ptr(), _ptr(stats), groups,
-                                  n // groups if groups else 0, cols, eps, TYPES[x.dtype], TYPES[x.dtype if wt is None else wt.dtype],
-                                  _stream(dev)), 'mgnn_layer_norm')
-  return y, x2, stats, weight
+  dy = dy.contiguous()
+  dx = torch.empty_like(dy) if want_x else None
+  dw = torch.empty(affine[0][0], dtype=affine[0][1], device=dev) if want_w else None
+  db = torch.empty(affine[1][0], dtype=affine[1][1], device=dev) if want_b else None
+  size = _workspace(*sizes, kinds[0]) if want_w or want_b else 0
+  room = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
+  _call(load().mgnn_layer_norm_backward, dev, x.data_ptr(), ld, dy.data_ptr(), w.data_ptr() if w is not None else None, stats.data_ptr(),
+        dx.data_ptr() if want_x else None, dw.data_ptr() if want_w else None, db.data_ptr() if want_b else None,
+        room.data_ptr() if size else None, size, *sizes, *kinds)
+  return dx, dw, db, None, None
+
+
+_ln_backward_once = once_differentiable(_ln_backward)
 
 
 class _LayerNorm(torch.autograd.Function):
 
   @staticmethod
   def forward(ctx, x, weight, bias, eps, groups):
-    y, x2, stats, w = _ln_forward(x, weight, bias, eps, groups, True)
+    y, x2, ld, stats, w, sizes, kinds = _ln_forward(x, weight, bias, eps, groups, True)
     ctx.save_for_backward(x2, stats, w)
-    ctx.groups, ctx.shape = groups, x.shape
-    ctx.affine = [None if t is None else (t.shape, t.dtype) for t in (weight, bias)]
+    ctx.plan = (ld, sizes, kinds, [None if t is None else (t.shape, t.dtype) for t in (weight, bias)])
     return y
 
   @staticmethod
-  @once_differentiable
   def backward(ctx, dy):
-    x2, stats, w = ctx.saved_tensors
-    want_x, want_w, want_b = ctx.needs_input_grad[:3]
-    dev, groups = x2.device, ctx.groups
-    n, cols = x2.shape
-    rows = n // groups if groups else 0
-    dy = dy.contiguous()
-    dx = torch.empty(ctx.shape, dtype=x2.dtype, device=dev) if want_x else None
-    dw, db = (torch.empty(s[0], dtype=s[1], device=dev) if want else None
-              for want, s in ((want_w, ctx.affine[0]), (want_b, ctx.affine[1])))
-    wt = next((s[1] for s in ctx.affine if s is not None), x2.dtype)
-    lib = load()
-    size = lib.mgnn_layer_norm_workspace(groups, rows, cols, TYPES[x2.dtype]) if want_w or want_b else 0
-    room = torch.empty(size // 4, dtype=torch.float32, device=dev) if size > 0 else None
-    with torch.cuda.device(dev):
-      _check(lib.mgnn_layer_norm_backward(x2.data_ptr(), x2.stride(0) if n > 1 else cols, dy.data_ptr(), _ptr(w), stats.data_ptr(),
-                                          _ptr(dx), _ptr(dw), _ptr(db), _ptr(room), size, groups, rows, cols, TYPES[x2.dtype],
-                                          TYPES[wt], _stream(dev)), 'mgnn_layer_norm_backward')
-    return dx, dw, db, None, None
+    # grad mode is on in here only under create_graph: then a second backward pass has to be refused
+    return _ln_backward_once(ctx, dy) if torch.is_grad_enabled() else _ln_backward(ctx, dy)
 
 
 def layer_norm(x, weight=None, bias=None, eps=1e-5):
@@ -188,7 +200,7 @@ def _grad_list(grads, stacked):
     raise ValueError('stacked is the length of the leading agent axis, 0 (none) to %d, not %r' % (MAX_GROUPS, stacked))
   dev = grads[0].device if grads else None
   for g in grads:
-    if g.dtype not in TYPES or g.layout != torch.strided:
+    if g.dtype not in TYPES or g.layout is not torch.strided:
       raise TypeError('gradients are dense float32, bfloat16 or float16 tensors, not %s, %s' % (g.dtype, g.layout))
     if g.device != dev:
       raise ValueError('gradients are on %s and %s: one device is wanted' % (dev, g.device))
@@ -199,31 +211,25 @@ def _grad_list(grads, stacked):
 
 def takes(grads):
   """Whether grads, a list, are what the kernels take: tensors on a GPU, of the types they know."""
-  return bool(grads) and all(g.is_cuda and g.dtype in TYPES and g.layout == torch.strided for g in grads)
-
-
-def _address(a):
-  return a.buffer_info()[0]
+  return bool(grads) and all(g.is_cuda and g.dtype in TYPES and g.layout is torch.strided for g in grads)
 
 
 def _launch(src, dst, max_norm, stacked, dev):
   """The kernels on dense tensors; dst None: the norms alone."""
-  lib, groups = load(), stacked or 1
-  count = len(src)
-  n = array.array('q', [t.numel() // groups for t in src])
+  lib, groups, count = load(), stacked or 1, len(src)
+  n = array.array('q', [t.numel() // groups for t in src] if stacked else [t.numel() for t in src])
   types = array.array('i', [TYPES[t.dtype] for t in src])
   sp = array.array('Q', [t.data_ptr() for t in src])
   norms = torch.empty((stacked,) if stacked else (), dtype=torch.float32, device=dev)
-  size = lib.mgnn_grad_norm_workspace(_address(n), _address(types), count, groups)
-  room = torch.empty(size // 8, dtype=torch.float64, device=dev) if size > 0 else None
-  with torch.cuda.device(dev):
-    if dst is None:
-      _check(lib.mgnn_grad_norm(_address(sp), _address(n), _address(types), count, groups, norms.data_ptr(), _ptr(room), size,
-                                _stream(dev)), 'mgnn_grad_norm')
-    else:
-      dp = array.array('Q', [t.data_ptr() for t in dst])
-      _check(lib.mgnn_clip_grads(_address(sp), _address(dp), _address(n), _address(types), count, groups, max_norm, norms.data_ptr(),
-                                 _ptr(room), size, _stream(dev)), 'mgnn_clip_grads')
+  np, tp = n.buffer_info()[0], types.buffer_info()[0]
+  size = lib.mgnn_grad_norm_workspace(np, tp, count, groups)
+  room = torch.empty(size, dtype=torch.uint8, device=dev) if size > 0 else None
+  work = room.data_ptr() if size > 0 else None
+  if dst is None:
+    _call(lib.mgnn_grad_norm, dev, sp.buffer_info()[0], np, tp, count, groups, norms.data_ptr(), work, size)
+  else:
+    dp = array.array('Q', [t.data_ptr() for t in dst])
+    _call(lib.mgnn_clip_grads, dev, sp.buffer_info()[0], dp.buffer_info()[0], np, tp, count, groups, max_norm, norms.data_ptr(), work, size)
   return norms
 
 
@@ -257,10 +263,13 @@ def clip_grads(grads, max_norm, stacked=0, out=None):
     out = [torch.empty_like(g) for g in grads]
   else:
     out = list(out)
-    if len(out) != len(grads) or any(o.shape != g.shape or o.dtype != g.dtype or o.device != g.device for o, g in zip(out, grads)):
-      raise ValueError('out does not match the gradients in number, shape, type or device')
-    if any(0 in [s for s, k in zip(o.stride(), o.shape) if k > 1] for o in out if not o.is_contiguous()):
-      raise ValueError('a gradient that is written has several elements at one address (an expanded tensor)')
+    if len(out) != len(grads):
+      raise ValueError('%d tensors in out for %d gradients' % (len(out), len(grads)))
+    for o, g in zip(out, grads):
+      if o is not g and (o.shape != g.shape or o.dtype != g.dtype or o.device != dev):
+        raise ValueError('out does not match the gradients in shape, type or device')
+      if not o.is_contiguous() and 0 in [s for s, k in zip(o.stride(), o.shape) if k > 1]:
+        raise ValueError('a gradient that is written has several elements at one address (an expanded tensor)')
   if dev is None or dev.type != 'cuda':
     norms = _plain_norms(grads, stacked)
     factor = (max_norm / (norms + 1e-6)).clamp(max=1.0).float()
@@ -269,7 +278,7 @@ def clip_grads(grads, max_norm, stacked=0, out=None):
     return out, norms.float()
   src, dst = [], []
   for g, o in zip(grads, out):
-    if g.is_contiguous() and o.is_contiguous() or (g.stride() == o.stride() and _dense(g, stacked)):
+    if (g.is_contiguous() and o.is_contiguous()) or (g.stride() == o.stride() and _dense(g, stacked)):
       src.append(g)
       dst.append(o)
     else:      # no common dense order: through contiguous copies
