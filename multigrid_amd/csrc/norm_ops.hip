@@ -24,6 +24,7 @@ struct Pack {
   typedef Vec VecAny __attribute__((aligned(sizeof(T))));
   static __device__ __forceinline__ Vec load(const T* p) { return *reinterpret_cast<const VecAny*>(p); }
   static __device__ __forceinline__ void store(T* p, Vec v) { *reinterpret_cast<VecAny*>(p) = v; }
+  static __device__ __forceinline__ void store_past_caches(T* p, Vec v) { __builtin_nontemporal_store(v, reinterpret_cast<VecAny*>(p)); }
 };
 
 // the vector at element `col` of a row of C elements; elements past the end (and whole vectors past it) are 0
@@ -400,6 +401,7 @@ __global__ __launch_bounds__(Shape<TPR>::BLOCK) void ln_bwd_kernel(const T* x, i
 
 // dweight / dbias of group blockIdx.y from the workgroups' shares, in a fixed order: 32 columns x 32 slices of the blocks
 constexpr int kJoinCols = 32, kJoinSlices = 32;
+static_assert(kJoinCols == kJoinSlices);      // the transposed read
 __global__ __launch_bounds__(kJoinCols* kJoinSlices) void ln_join_kernel(const float* partial, int blocks, int C, void* dweight,
                                                                          void* dbias, int wtype) {
   __shared__ float red[kJoinSlices][kJoinCols + 1];
@@ -408,18 +410,18 @@ __global__ __launch_bounds__(kJoinCols* kJoinSlices) void ln_join_kernel(const f
   const int64_t col = (int64_t)blockIdx.x * kJoinCols + c;
   float acc = 0.f;
   if (col < 2 * C) {
-#pragma unroll 8
-    for (int k = s; k < blocks; k += kJoinSlices) acc += partial[(g * blocks + k) * 2 * C + col];
+    const float* p = partial + g * blocks * 2 * C + col;
+#pragma unroll 16
+    for (int k = s; k < blocks; k += kJoinSlices) acc += p[(int64_t)k * 2 * C];
   }
   red[s][c] = acc;
   __syncthreads();
-  for (int half = kJoinSlices / 2; half >= 1; half >>= 1) {
-    if (s < half) red[s][c] += red[s + half][c];
-    __syncthreads();
-  }
-  if (s == 0 && col < 2 * C) {
-    void* out = col < C ? dweight : dbias;
-    if (out) store_from_float(out, wtype, g * C + (col < C ? col : col - C), red[0][c]);
+  // now 32 lanes of a wave hold a column's slices
+  const float sum = lanes_sum<kJoinSlices>(red[c][s]);
+  const int64_t out_col = (int64_t)blockIdx.x * kJoinCols + s;
+  if (c == 0 && out_col < 2 * C) {
+    void* out = out_col < C ? dweight : dbias;
+    if (out) store_from_float(out, wtype, g * C + (out_col < C ? out_col : out_col - C), sum);
   }
 }
 
@@ -574,7 +576,7 @@ __device__ __forceinline__ double chunk_squares(const T* p, int64_t n) {      //
   return acc;
 }
 
-__global__ __launch_bounds__(kBlock) void grad_squares_kernel(GradTable t, double* partial, int row, int rows_of_group) {
+__global__ __launch_bounds__(kBlock, 8) void grad_squares_kernel(GradTable t, double* partial, int row, int rows_of_group) {
   __shared__ double lds[kBlock / kWave];
   const int64_t g = blockIdx.y;
   const int chunks = t.end[t.count - 1];
@@ -616,22 +618,23 @@ __global__ __launch_bounds__(kBlock) void grad_norm_kernel(const double* partial
 }
 
 template <typename T>
-__device__ __forceinline__ void chunk_scale(const T* p, T* q, int64_t n, float f) {
+__device__ __forceinline__ void chunk_scale(const T* p, T* q, int64_t n, float f, bool past_caches) {
   constexpr int V = Pack<T>::V;
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
-    const int at = (u * kBlock + threadIdx.x) * V;
+    const int at = (u * kBlock + threadIdx.x) * V, end = (int)min(n, (int64_t)kChunkBytes);
     if (at < n) {
-      typename Pack<T>::Vec v = load_part(p, at, (int)min(n, (int64_t)kChunkBytes));
+      typename Pack<T>::Vec v = load_part(p, at, end);
 #pragma unroll
       for (int k = 0; k < V; ++k) v[k] = (T)((float)v[k] * f);
-      store_part(q, at, (int)min(n, (int64_t)kChunkBytes), v);
+      if (past_caches && at + V <= end) Pack<T>::store_past_caches(q + at, v);
+      else store_part(q, at, end, v);
     }
   }
 }
 
-__global__ __launch_bounds__(kBlock) void grad_scale_kernel(GradTable t, const double* partial, int rows_of_group, double max_norm,
-                                                            float* norms) {
+__global__ __launch_bounds__(kBlock, 8) void grad_scale_kernel(GradTable t, const double* partial, int rows_of_group, double max_norm,
+                                                            float* norms, bool past_caches) {
   __shared__ double lds[kBlock / kWave];
   __shared__ float factor;
   const int64_t g = blockIdx.y;
@@ -644,9 +647,10 @@ __global__ __launch_bounds__(kBlock) void grad_scale_kernel(GradTable t, const d
     if (f == 1.f && t.src[i] == t.dst[i]) continue;      // a factor of 1 in place: nothing changes
     const int64_t at = (int64_t)(c - (i ? t.end[i - 1] : 0)) * (kChunkBytes / (t.type[i] == MGNN_F32 ? 4 : 2));
     const int64_t off = g * t.n[i] + at, n = t.n[i] - at;
-    if (t.type[i] == MGNN_F32) chunk_scale(static_cast<const float*>(t.src[i]) + off, static_cast<float*>(t.dst[i]) + off, n, f);
-    else if (t.type[i] == MGNN_BF16) chunk_scale(static_cast<const __bf16*>(t.src[i]) + off, static_cast<__bf16*>(t.dst[i]) + off, n, f);
-    else chunk_scale(static_cast<const _Float16*>(t.src[i]) + off, static_cast<_Float16*>(t.dst[i]) + off, n, f);
+    if (t.type[i] == MGNN_F32) chunk_scale(static_cast<const float*>(t.src[i]) + off, static_cast<float*>(t.dst[i]) + off, n, f, past_caches);
+    else if (t.type[i] == MGNN_BF16)
+      chunk_scale(static_cast<const __bf16*>(t.src[i]) + off, static_cast<__bf16*>(t.dst[i]) + off, n, f, past_caches);
+    else chunk_scale(static_cast<const _Float16*>(t.src[i]) + off, static_cast<_Float16*>(t.dst[i]) + off, n, f, past_caches);
   }
 }
 
@@ -842,7 +846,9 @@ int grad_plan(const void* const* src, void* const* dst, const int64_t* n, const 
     }
   }
   for (const GradTable& t : plan.tables) {
-    const int64_t cap = std::max<int64_t>(1, 1024 / groups);
+    // as many workgroups as stand on the card at once, eight per CU, so that none starts late (2.1 GB of fp32, at 80 registers
+    // and 1536 / 2048 workgroups: 1131 / 1277 us, at 64 registers: 1130 / 1113)
+    const int64_t cap = std::max<int64_t>(1, 2048 / groups);
     plan.blocks.push_back((int)std::min<int64_t>(t.end[t.count - 1], cap));
     plan.rows += plan.blocks.back();
   }
@@ -908,9 +914,15 @@ int clip(const void* const* src, void* const* dst, const int64_t* n, const int32
     hipLaunchKernelGGL(grad_norm_kernel, dim3((unsigned)groups), dim3(kBlock), 0, stream, partial, plan.rows, norms);
     return launched();
   }
+  // Results of more than the 256 MB of the memory-side cache go past it: they would push out the gradients that are still
+  // to be read, and the next reader would not find them there either (256 MB of bf16 apart: 153 -> 131 us, with a copy of
+  // the results behind it 350 -> 348).
+  int64_t bytes = 0;
+  for (int64_t i = 0; i < count; ++i) bytes += n[i] * groups * elem_bytes(type[i]);
+  const bool past_caches = bytes >= (int64_t)256 << 20;
   for (size_t k = plan.tables.size(); k-- > 0;)
     hipLaunchKernelGGL(grad_scale_kernel, dim3(plan.blocks[k], (unsigned)groups), dim3(kBlock), 0, stream, plan.tables[k], partial,
-                       plan.rows, max_norm, k == 0 ? norms : nullptr);
+                       plan.rows, max_norm, k == 0 ? norms : nullptr, past_caches);
   return launched();
 }
 

@@ -13,6 +13,7 @@ import array
 import ctypes as C
 import functools
 import math
+import operator
 
 import torch
 import torch.nn.functional as F
@@ -68,26 +69,29 @@ def _call(fn, dev, *args):
 
 def _ln_args(x, weight, bias, eps):
   """The number of weight rows (1, or the leading axis of x)."""
-  if x.dtype not in TYPES or x.layout != torch.strided:
+  if x.dtype not in TYPES or x.layout is not torch.strided:
     raise TypeError('layer_norm takes dense float32, bfloat16 or float16 tensors, not %s' % x.dtype)
-  if x.dim() < 1 or not 1 <= x.shape[-1] <= MAX_COLS:
+  if x.dim() < 1 or not 1 <= x.size(-1) <= MAX_COLS:
     raise ValueError('layer_norm takes rows of 1 to %d elements, not a tensor of shape %s' % (MAX_COLS, tuple(x.shape)))
-  if not eps >= 0 or math.isinf(eps):
+  if not 0 <= eps < math.inf:
     raise ValueError('layer_norm takes a finite eps >= 0, not %r' % (eps,))
   groups = 1
-  for name, t in (('weight', weight), ('bias', bias)):
+  for t in (weight, bias):
     if t is None:
       continue
-    if t.dtype not in (x.dtype, torch.float32) or t.layout != torch.strided:
-      raise TypeError("layer_norm's %s is %s: x's type (%s) or float32 is wanted" % (name, t.dtype, x.dtype))
+    if t.dtype not in (x.dtype, torch.float32) or t.layout is not torch.strided:
+      raise TypeError("layer_norm's weight and bias are of x's type (%s) or float32, not %s" % (x.dtype, t.dtype))
     if t.device != x.device:
-      raise ValueError("layer_norm's %s is on %s, x on %s" % (name, t.device, x.device))
-    stacked = t.dim() == 2 and x.dim() >= 2 and t.shape[0] == x.shape[0]
-    if t.shape[-1:] != x.shape[-1:] or not (t.dim() == 1 or stacked):
-      raise ValueError("layer_norm's %s of shape %s does not fit x of shape %s: [cols] or [x.shape[0], cols] is wanted"
-                       % (name, tuple(t.shape), tuple(x.shape)))
-    groups = t.shape[0] if stacked else 1
-  if weight is not None and bias is not None and (weight.shape != bias.shape or weight.dtype != bias.dtype):
+      raise ValueError("layer_norm's weight and bias are on %s, x on %s" % (t.device, x.device))
+    shape = t.shape
+    if len(shape) == 2 and x.dim() >= 2 and shape[0] == x.size(0):
+      groups = shape[0]
+    elif len(shape) != 1:
+      shape = ()
+    if not shape or shape[-1] != x.size(-1):
+      raise ValueError("layer_norm's weight or bias of shape %s does not fit x of shape %s: [cols] or [x.shape[0], cols] is wanted"
+                       % (tuple(t.shape), tuple(x.shape)))
+  if weight is not None and bias is not None and (weight.dtype != bias.dtype or weight.shape != bias.shape):
     raise ValueError("layer_norm's weight and bias differ in shape or type")
   if groups > MAX_GROUPS:
     raise ValueError('layer_norm takes at most %d weight rows, not %d' % (MAX_GROUPS, groups))
@@ -132,13 +136,13 @@ def _ln_forward(x, weight, bias, eps, groups, want_stats):
 
 def _ln_backward(ctx, dy):
   x, stats, w = ctx.saved_tensors
-  ld, sizes, kinds, affine = ctx.plan
+  ld, sizes, kinds, bias = ctx.plan
   want_x, want_w, want_b = ctx.needs_input_grad[:3]
   dev = x.device
   dy = dy.contiguous()
   dx = torch.empty_like(dy) if want_x else None
-  dw = torch.empty(affine[0][0], dtype=affine[0][1], device=dev) if want_w else None
-  db = torch.empty(affine[1][0], dtype=affine[1][1], device=dev) if want_b else None
+  dw = torch.empty_like(w) if want_w else None
+  db = (torch.empty_like(w) if w is not None else torch.empty(bias[0], dtype=bias[1], device=dev)) if want_b else None
   size = _workspace(*sizes, kinds[0]) if want_w or want_b else 0
   room = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
   _call(load().mgnn_layer_norm_backward, dev, x.data_ptr(), ld, dy.data_ptr(), w.data_ptr() if w is not None else None, stats.data_ptr(),
@@ -156,7 +160,7 @@ class _LayerNorm(torch.autograd.Function):
   def forward(ctx, x, weight, bias, eps, groups):
     y, x2, ld, stats, w, sizes, kinds = _ln_forward(x, weight, bias, eps, groups, True)
     ctx.save_for_backward(x2, stats, w)
-    ctx.plan = (ld, sizes, kinds, [None if t is None else (t.shape, t.dtype) for t in (weight, bias)])
+    ctx.plan = (ld, sizes, kinds, (bias.shape, bias.dtype) if weight is None and bias is not None else None)
     return y
 
   @staticmethod
@@ -199,13 +203,15 @@ def _grad_list(grads, stacked):
   if not isinstance(stacked, int) or not 0 <= stacked <= MAX_GROUPS:
     raise ValueError('stacked is the length of the leading agent axis, 0 (none) to %d, not %r' % (MAX_GROUPS, stacked))
   dev = grads[0].device if grads else None
-  for g in grads:
-    if g.dtype not in TYPES or g.layout is not torch.strided:
-      raise TypeError('gradients are dense float32, bfloat16 or float16 tensors, not %s, %s' % (g.dtype, g.layout))
-    if g.device != dev:
-      raise ValueError('gradients are on %s and %s: one device is wanted' % (dev, g.device))
-    if stacked and (g.dim() < 1 or g.shape[0] != stacked):
-      raise ValueError('a gradient of shape %s has no leading agent axis of %d' % (tuple(g.shape), stacked))
+  for kind in {(g.dtype, g.layout) for g in grads}:
+    if kind[0] not in TYPES or kind[1] is not torch.strided:
+      raise TypeError('gradients are dense float32, bfloat16 or float16 tensors, not %s, %s' % kind)
+  if len({g.device for g in grads}) > 1:
+    raise ValueError('gradients are on several devices: %s' % ', '.join(sorted({str(g.device) for g in grads})))
+  if stacked:
+    for g in grads:
+      if g.dim() < 1 or g.size(0) != stacked:
+        raise ValueError('a gradient of shape %s has no leading agent axis of %d' % (tuple(g.shape), stacked))
   return grads, dev
 
 
@@ -228,7 +234,7 @@ def _launch(src, dst, max_norm, stacked, dev):
   if dst is None:
     _call(lib.mgnn_grad_norm, dev, sp.buffer_info()[0], np, tp, count, groups, norms.data_ptr(), work, size)
   else:
-    dp = array.array('Q', [t.data_ptr() for t in dst])
+    dp = sp if dst is src else array.array('Q', [t.data_ptr() for t in dst])
     _call(lib.mgnn_clip_grads, dev, sp.buffer_info()[0], dp.buffer_info()[0], np, tp, count, groups, max_norm, norms.data_ptr(), work, size)
   return norms
 
@@ -259,36 +265,40 @@ def clip_grads(grads, max_norm, stacked=0, out=None):
   max_norm = float(max_norm)
   if not max_norm >= 0:
     raise ValueError('max_norm is a number >= 0, not %r' % max_norm)
+  plain = all([g.is_contiguous() for g in grads])      # every tensor of the call
   if out is None:
     out = [torch.empty_like(g) for g in grads]
   else:
     out = list(out)
-    if len(out) != len(grads):
-      raise ValueError('%d tensors in out for %d gradients' % (len(out), len(grads)))
-    for o, g in zip(out, grads):
-      if o is not g and (o.shape != g.shape or o.dtype != g.dtype or o.device != dev):
-        raise ValueError('out does not match the gradients in shape, type or device')
-      if not o.is_contiguous() and 0 in [s for s, k in zip(o.stride(), o.shape) if k > 1]:
-        raise ValueError('a gradient that is written has several elements at one address (an expanded tensor)')
+    apart = len(out) != len(grads) or not all(map(operator.is_, out, grads))
+    if apart and ([o.shape for o in out] != [g.shape for g in grads] or [o.dtype for o in out] != [g.dtype for g in grads]
+                  or any([o.device != dev for o in out])):
+      raise ValueError('out does not match the gradients in number, shape, type or device')
+    plain = plain and (not apart or all([o.is_contiguous() for o in out]))
+    if not plain and any(0 in [s for s, k in zip(o.stride(), o.shape) if k > 1] for o in out):
+      raise ValueError('a gradient that is written has several elements at one address (an expanded tensor)')
   if dev is None or dev.type != 'cuda':
     norms = _plain_norms(grads, stacked)
     factor = (max_norm / (norms + 1e-6)).clamp(max=1.0).float()
     for o, g in zip(out, grads):
       o.copy_(g.float() * factor.reshape(factor.shape + (1,) * (g.dim() - factor.dim())))
     return out, norms.float()
-  src, dst = [], []
-  for g, o in zip(grads, out):
-    if (g.is_contiguous() and o.is_contiguous()) or (g.stride() == o.stride() and _dense(g, stacked)):
-      src.append(g)
-      dst.append(o)
-    else:      # no common dense order: through contiguous copies
-      src.append(g.contiguous())
-      dst.append(src[-1] if o is g else torch.empty(o.shape, dtype=o.dtype, device=dev))
+  src, dst = grads, out
+  if not plain:
+    src, dst = [], []
+    for g, o in zip(grads, out):
+      if (g.is_contiguous() and o.is_contiguous()) or (g.stride() == o.stride() and _dense(g, stacked)):
+        src.append(g)
+        dst.append(o)
+      else:      # no common dense order: through contiguous copies
+        src.append(g.contiguous())
+        dst.append(torch.empty(o.shape, dtype=o.dtype, device=dev))
   norms = _launch(src, dst, max_norm, stacked, dev)
   torch.autograd.graph.increment_version(dst)      # written behind autograd's back: a graph that saved one of them will say so
-  for d, o in zip(dst, out):
-    if d is not o:
-      o.copy_(d)
+  if not plain:
+    for d, o in zip(dst, out):
+      if d is not o:
+        o.copy_(d)
   return out, norms
 
 
