@@ -1,0 +1,269 @@
+// The torch side of include/mgrid_norm.h: argument checks, autograd and memory of layer_norm, grad_norm and clip_grads, with
+// the plain torch expression of the same formulas for tensors that are not on a GPU.  multigrid_amd/norm_ops.py documents and
+// re-exports them.  In C++ because the smallest calls are bound by their host time: the autograd graph's nodes, the
+// allocations and a list of gradients cost several times as much from Python (forward and backward of a small layer norm
+// 98 us from Python; a list of 36 gradients 47 us).
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/utils/pybind.h>
+
+#include <cmath>
+#include <optional>
+#include <tuple>
+#include <vector>
+
+#include "mgrid_norm.h"
+
+namespace {
+
+using at::Tensor;
+using MaybeTensor = std::optional<Tensor>;
+
+// the kernels' number of an element type; -1: none
+int type_of(const Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return MGNN_F32;
+    case at::kBFloat16: return MGNN_BF16;
+    case at::kHalf: return MGNN_F16;
+    default: return -1;
+  }
+}
+bool takes(const Tensor& t) { return type_of(t) >= 0 && t.layout() == at::kStrided; }
+
+void check(int rc, const char* what) {
+  TORCH_CHECK(rc != MGNN_ERR_LAUNCH, what, ": the kernel launch failed");
+  TORCH_CHECK_VALUE(rc != MGNN_ERR_OVERLAP, what, ": a gradient that is written overlaps another one of the call");
+  TORCH_CHECK_VALUE(rc == MGNN_OK, what, ": refused with MGNN error ", rc);
+}
+
+void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+
+Tensor bytes_on(const Tensor& t, int64_t size) { return size > 0 ? at::empty({size}, t.options().dtype(at::kByte)) : Tensor(); }
+void* data(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// ---- layer norm ----
+
+// x by rows (x itself, a view of it, or a copy) with the elements of a row contiguous, and the distance of its rows
+std::pair<Tensor, int64_t> rows_of(const Tensor& x, int64_t cols) {
+  if (x.is_contiguous()) return {x, cols};
+  Tensor r = x.reshape({-1, cols});
+  if ((cols > 1 && r.stride(1) != 1) || (r.size(0) > 1 && r.stride(0) < cols)) return {r.contiguous(), cols};
+  return {r, r.size(0) > 1 ? r.stride(0) : cols};
+}
+
+struct Sizes {
+  int64_t groups, rows, cols;
+  int type, wtype;
+};
+
+Tensor forward_kernel(const Tensor& x, int64_t ld, at::IntArrayRef shape, const Tensor& w, const Tensor& b, const Tensor& stats, double eps,
+                      const Sizes& s) {
+  Tensor y = at::empty(shape, x.options());
+  check(mgnn_layer_norm(x.data_ptr(), ld, data(w), data(b), y.data_ptr(), stats.defined() ? stats.data_ptr<float>() : nullptr, s.groups, s.rows,
+                        (int)s.cols, eps, s.type, s.wtype, stream_of(x)),
+        "layer_norm");
+  return y;
+}
+
+struct LayerNorm : public torch::autograd::Function<LayerNorm> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps,
+                        const Sizes& s) {
+    const auto [rows, ld] = rows_of(x, s.cols);
+    const Tensor w = weight ? weight->contiguous() : Tensor(), b = bias ? bias->contiguous() : Tensor();
+    const Tensor stats = at::empty({s.groups * s.rows, 2}, x.options().dtype(at::kFloat));
+    Tensor y = forward_kernel(rows, ld, x.sizes(), w, b, stats, eps, s);
+    ctx->save_for_backward({rows, stats, w});
+    ctx->saved_data["ld"] = ld;
+    ctx->saved_data["sizes"] = std::vector<int64_t>{s.groups, s.rows, s.cols, s.type, s.wtype};
+    ctx->saved_data["affine"] = std::vector<int64_t>{weight.has_value(), bias.has_value(), weight ? weight->dim() : bias ? bias->dim() : 0};
+    return y;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "layer_norm is differentiable once: its gradients have no graph (create_graph)");
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &stats = saved[1], &w = saved[2];
+    const int64_t ld = ctx->saved_data["ld"].toInt();
+    const auto n = ctx->saved_data["sizes"].toIntVector(), affine = ctx->saved_data["affine"].toIntVector();
+    const Sizes s{n[0], n[1], n[2], (int)n[3], (int)n[4]};
+    const c10::DeviceGuard guard(x.device());
+    const Tensor dy = grads[0].contiguous();
+    // the node's edges are those of the tensors that were given
+    const bool want_w = affine[0] && ctx->needs_input_grad(1), want_b = affine[1] && ctx->needs_input_grad(affine[0] ? 2 : 1);
+    Tensor dx, dw, db;
+    if (ctx->needs_input_grad(0)) dx = at::empty_like(dy);
+    const auto row_shape = affine[2] == 2 ? std::vector<int64_t>{s.groups, s.cols} : std::vector<int64_t>{s.cols};
+    const auto row_options = x.options().dtype(s.wtype == MGNN_F32 ? at::kFloat : x.scalar_type());
+    if (want_w) dw = at::empty(row_shape, row_options);
+    if (want_b) db = at::empty(row_shape, row_options);
+    const int64_t size = want_w || want_b ? mgnn_layer_norm_workspace(s.groups, s.rows, (int)s.cols, s.type) : 0;
+    const Tensor room = bytes_on(x, size);
+    check(mgnn_layer_norm_backward(x.data_ptr(), ld, dy.data_ptr(), data(w), stats.data_ptr<float>(), data(dx), data(dw), data(db), data(room),
+                                   size, s.groups, s.rows, (int)s.cols, s.type, s.wtype, stream_of(x)),
+          "layer_norm's backward pass");
+    return {dx, dw, db, Tensor(), Tensor()};
+  }
+};
+
+Tensor plain_layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps) {
+  const auto row = [&](const Tensor& t) {      // a stacked weight against x
+    if (t.dim() == 1) return t.to(at::kFloat);
+    std::vector<int64_t> shape(x.dim(), 1);
+    shape.front() = x.size(0);
+    shape.back() = x.size(-1);
+    return t.to(at::kFloat).reshape(shape);
+  };
+  Tensor h = at::layer_norm(x.to(at::kFloat), {x.size(-1)}, {}, {}, eps);
+  if (weight) h = h * row(*weight);
+  if (bias) h = h + row(*bias);
+  return h.to(x.scalar_type());
+}
+
+Tensor layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor& bias, double eps) {
+  TORCH_CHECK_TYPE(takes(x), "layer_norm takes dense float32, bfloat16 or float16 tensors, not ", x.scalar_type(), ", ", x.layout());
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) >= 1 && x.size(-1) <= MGNN_LN_MAX_C, "layer_norm takes rows of 1 to ", MGNN_LN_MAX_C,
+                    " elements, not a tensor of shape ", x.sizes());
+  TORCH_CHECK_VALUE(eps >= 0 && !std::isinf(eps), "layer_norm takes a finite eps >= 0, not ", eps);
+  Sizes s{1, 0, x.size(-1), type_of(x), type_of(x)};
+  for (const MaybeTensor* p : {&weight, &bias}) {
+    if (!*p) continue;
+    const Tensor& t = **p;
+    TORCH_CHECK_TYPE(takes(t) && (t.scalar_type() == x.scalar_type() || t.scalar_type() == at::kFloat),
+                     "layer_norm's weight and bias are dense, of x's type (", x.scalar_type(), ") or float32, not ", t.scalar_type());
+    TORCH_CHECK_VALUE(t.device() == x.device(), "layer_norm's weight and bias are on ", t.device(), ", x on ", x.device());
+    const bool stacked = t.dim() == 2 && x.dim() >= 2 && t.size(0) == x.size(0);
+    TORCH_CHECK_VALUE((t.dim() == 1 || stacked) && t.size(-1) == s.cols, "layer_norm's weight or bias of shape ", t.sizes(),
+                      " does not fit x of shape ", x.sizes(), ": [cols] or [x.shape[0], cols] is wanted");
+    if (stacked) s.groups = t.size(0);
+    s.wtype = type_of(t);
+  }
+  TORCH_CHECK_VALUE(!weight || !bias || (weight->sizes() == bias->sizes() && weight->scalar_type() == bias->scalar_type()),
+                    "layer_norm's weight and bias differ in shape or type");
+  TORCH_CHECK_VALUE(s.groups <= MGNN_MAX_GROUPS, "layer_norm takes at most ", MGNN_MAX_GROUPS, " weight rows, not ", s.groups);
+  if (!x.is_cuda()) return plain_layer_norm(x, weight, bias, eps);
+  s.rows = s.groups ? x.numel() / s.cols / s.groups : 0;
+  const c10::DeviceGuard guard(x.device());
+  if (at::GradMode::is_enabled() && (x.requires_grad() || (weight && weight->requires_grad()) || (bias && bias->requires_grad())))
+    return LayerNorm::apply(x, weight, bias, eps, s);
+  const auto [rows, ld] = rows_of(x, s.cols);
+  return forward_kernel(rows, ld, x.sizes(), weight ? weight->contiguous() : Tensor(), bias ? bias->contiguous() : Tensor(), Tensor(), eps, s);
+}
+
+// ---- the global gradient norm ----
+
+using Tensors = std::vector<Tensor>;
+
+// Whether t's elements fill one stretch of memory, in whatever order (stacked: agent by agent)
+bool dense(const Tensor& t, bool stacked) {
+  return t.is_contiguous() || (t.is_non_overlapping_and_dense() && (!stacked || t.size(0) == 1 || t.stride(0) == t.numel() / t.size(0)));
+}
+
+void check_grads(const Tensors& grads, int64_t stacked) {
+  TORCH_CHECK_VALUE(stacked >= 0 && stacked <= MGNN_MAX_GROUPS, "stacked is the length of the leading agent axis, 0 (none) to ", MGNN_MAX_GROUPS,
+                    ", not ", stacked);
+  for (const Tensor& g : grads) {
+    TORCH_CHECK_TYPE(takes(g), "gradients are dense float32, bfloat16 or float16 tensors, not ", g.scalar_type(), ", ", g.layout());
+    TORCH_CHECK_VALUE(g.device() == grads[0].device(), "gradients are on ", grads[0].device(), " and ", g.device(), ": one device is wanted");
+    TORCH_CHECK_VALUE(!stacked || (g.dim() >= 1 && g.size(0) == stacked), "a gradient of shape ", g.sizes(), " has no leading agent axis of ",
+                      stacked);
+  }
+}
+
+std::vector<int64_t> norm_shape(int64_t stacked) { return stacked ? std::vector<int64_t>{stacked} : std::vector<int64_t>{}; }
+
+Tensor plain_norms(const Tensors& grads, int64_t stacked) {      // float64
+  Tensor sum = grads.empty() ? at::zeros(norm_shape(stacked), at::kDouble) : at::zeros(norm_shape(stacked), grads[0].options().dtype(at::kDouble));
+  for (const Tensor& g : grads) {
+    const Tensor sq = g.to(at::kDouble).square();
+    sum = sum + (stacked ? sq.reshape({stacked, -1}).sum(1) : sq.sum());
+  }
+  return sum.sqrt();
+}
+
+// The kernels on dense tensors; dst NULL: the norms alone
+Tensor launch(const Tensors& src, const Tensors* dst, double max_norm, int64_t stacked) {
+  const int64_t groups = std::max<int64_t>(stacked, 1), count = (int64_t)src.size();
+  std::vector<const void*> from(count);
+  std::vector<void*> to(count);
+  std::vector<int64_t> n(count);
+  std::vector<int32_t> type(count);
+  for (int64_t i = 0; i < count; ++i) {
+    from[i] = src[i].data_ptr();
+    if (dst) to[i] = (*dst)[i].data_ptr();
+    n[i] = src[i].numel() / groups;
+    type[i] = type_of(src[i]);
+  }
+  const c10::DeviceGuard guard(src[0].device());
+  Tensor norms = at::empty(norm_shape(stacked), src[0].options().dtype(at::kFloat));
+  const int64_t size = mgnn_grad_norm_workspace(n.data(), type.data(), count, groups);
+  const Tensor room = bytes_on(src[0], size);
+  void* const stream = stream_of(src[0]);
+  check(dst ? mgnn_clip_grads(from.data(), to.data(), n.data(), type.data(), count, groups, max_norm, norms.data_ptr<float>(), data(room), size,
+                              stream)
+            : mgnn_grad_norm(from.data(), n.data(), type.data(), count, groups, norms.data_ptr<float>(), data(room), size, stream),
+        dst ? "clip_grads" : "grad_norm");
+  return norms;
+}
+
+Tensor grad_norm(const Tensors& grads, int64_t stacked) {
+  const at::NoGradGuard no_grad;
+  check_grads(grads, stacked);
+  if (grads.empty() || !grads[0].is_cuda()) return plain_norms(grads, stacked).to(at::kFloat);
+  Tensors src;
+  for (const Tensor& g : grads) src.push_back(dense(g, stacked) ? g : g.contiguous());
+  return launch(src, nullptr, 0.0, stacked);
+}
+
+std::tuple<Tensors, Tensor> clip_grads(const Tensors& grads, double max_norm, int64_t stacked, const std::optional<Tensors>& given) {
+  const at::NoGradGuard no_grad;
+  check_grads(grads, stacked);
+  TORCH_CHECK_VALUE(max_norm >= 0, "max_norm is a number >= 0, not ", max_norm);
+  const size_t count = grads.size();
+  Tensors out;
+  if (given) {
+    TORCH_CHECK_VALUE(given->size() == count, given->size(), " tensors in out for ", count, " gradients");
+    out = *given;
+    for (size_t i = 0; i < count; ++i) {
+      const Tensor &o = out[i], &g = grads[i];
+      TORCH_CHECK_VALUE(o.sizes() == g.sizes() && o.scalar_type() == g.scalar_type() && o.device() == g.device() && o.layout() == at::kStrided,
+                        "out does not match the gradients in shape, type or device");
+      for (int64_t d = 0; d < o.dim() && !o.is_contiguous(); ++d)
+        TORCH_CHECK_VALUE(o.size(d) <= 1 || o.stride(d) != 0, "a gradient that is written has several elements at one address (an expanded tensor)");
+    }
+  } else {
+    for (const Tensor& g : grads) out.push_back(at::empty_like(g));
+  }
+  if (count == 0 || !grads[0].is_cuda()) {
+    const Tensor norms = plain_norms(grads, stacked), factor = (max_norm / (norms + 1e-6)).clamp_max(1.0).to(at::kFloat);
+    for (size_t i = 0; i < count; ++i) {
+      std::vector<int64_t> wide(grads[i].dim(), 1);
+      if (stacked) wide[0] = stacked;
+      out[i].copy_(grads[i].to(at::kFloat) * (stacked ? factor.reshape(wide) : factor));
+    }
+    return {out, norms.to(at::kFloat)};
+  }
+  // tensors without a common dense order go through contiguous copies
+  Tensors src(grads), dst(out);
+  for (size_t i = 0; i < count; ++i) {
+    if ((src[i].is_contiguous() && dst[i].is_contiguous()) || (src[i].strides() == dst[i].strides() && dense(src[i], stacked))) continue;
+    src[i] = src[i].contiguous();
+    dst[i] = at::empty(out[i].sizes(), out[i].options());
+  }
+  const Tensor norms = launch(src, &dst, max_norm, stacked);
+  for (size_t i = 0; i < count; ++i) {
+    if (!dst[i].is_same(out[i])) out[i].copy_(dst[i]);
+    else if (!out[i].is_inference()) out[i].unsafeGetTensorImpl()->bump_version();      // a graph that saved it will say so
+  }
+  return {out, norms};
+}
+
+}  // namespace
+
+PYBIND11_MODULE(_norm_ops, m) {
+  namespace py = pybind11;
+  m.def("layer_norm", &layer_norm, py::arg("x"), py::arg("weight") = py::none(), py::arg("bias") = py::none(), py::arg("eps") = 1e-5);
+  m.def("grad_norm", &grad_norm, py::arg("grads"), py::arg("stacked") = 0);
+  m.def("clip_grads", &clip_grads, py::arg("grads"), py::arg("max_norm"), py::arg("stacked") = 0, py::arg("out") = py::none());
+}

@@ -7,6 +7,7 @@ below 40 u times the row's mean |x|; the sum of squared deviations likewise 40 u
 import pytest
 import torch
 
+import norm_abi
 from multigrid_amd import norm_ops, ppo
 
 pytestmark = pytest.mark.gpu
@@ -153,7 +154,7 @@ def test_layouts_of_the_input(dtype):
 
 def test_nothing_behind_the_rows_is_written():
   """Outputs through the C ABI into the middle of a larger buffer of a known value: its other elements keep it."""
-  lib = norm_ops.load()
+  lib = norm_abi.load()
   stream = torch.cuda.current_stream().cuda_stream
   for dtype, cols, rows in ((F32, 13, 5), (BF16, 37, 70), (F16, 2051, 3), (F32, 16381, 2), (F16, 1, 9)):
     t, n = norm_ops.TYPES[dtype], rows * cols

@@ -8,6 +8,7 @@ import re
 import pytest
 import torch
 
+import norm_abi
 from multigrid_amd import norm_ops, ppo
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
@@ -20,8 +21,8 @@ def _header():
 def test_every_declared_symbol_is_exported_and_bound():
   src = _header()
   names = sorted(set(re.findall(r'\b(mgnn_[a-z_0-9]+)\s*\(', src)))
-  assert sorted(norm_ops.SYMBOLS) == names
-  lib = norm_ops.load()
+  assert sorted(norm_abi.SYMBOLS) == names
+  lib = norm_abi.load()
   assert all(hasattr(lib, n) for n in names)
   define = dict(re.findall(r'#define (\w+) (\d+)', src))
   assert int(define['MGNN_LN_MAX_C']) == norm_ops.MAX_COLS and int(define['MGNN_MAX_GROUPS']) == norm_ops.MAX_GROUPS
@@ -34,7 +35,7 @@ def _list(ns, types):
 
 
 def test_layer_norm_entry_points_refuse_before_any_launch():
-  lib = norm_ops.load()
+  lib = norm_abi.load()
   shape, typ, ws, val = 1, 3, 4, 5
   one = C.c_void_p(16)      # never dereferenced: refused first
 
@@ -60,7 +61,7 @@ def test_layer_norm_entry_points_refuse_before_any_launch():
 
 
 def test_gradient_entry_points_refuse_before_any_launch():
-  lib = norm_ops.load()
+  lib = norm_abi.load()
   shape, typ, ws, val, over = 1, 3, 4, 5, 6
   one = C.c_void_p(16)
 
@@ -124,7 +125,7 @@ def test_gradient_refusals():
   a, b = torch.ones(3, 4), torch.ones(3)
   for grads, stacked, error in (([a.double()], 0, TypeError), ([a.int()], 0, TypeError), ([a.to_sparse()], 0, TypeError),
                                 ([a, torch.ones(3, device='meta')], 0, ValueError), ([a, torch.ones(2)], 3, ValueError),
-                                ([torch.ones(())], 1, ValueError), ([a], -1, ValueError), ([a], 1.5, ValueError),
+                                ([torch.ones(())], 1, ValueError), ([a], -1, ValueError), ([a], 1.5, TypeError), ([a, None], 0, TypeError),
                                 ([a], norm_ops.MAX_GROUPS + 1, ValueError)):
     with pytest.raises(error):
       norm_ops.grad_norm(grads, stacked)
