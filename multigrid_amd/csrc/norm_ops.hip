@@ -452,24 +452,35 @@ int64_t even_blocks(int64_t want, int64_t groups, int64_t most) {
   return steps ? (want + steps - 1) / steps : 1;
 }
 
-// Forward: workgroups stay, keep their weight rows in registers and load the next row under the sums of this one.  16 waves
-// per CU carry fp32 rows (3 x 409600 rows of 128: 229 us, 8 waves 294, 32 waves 249) and rows over several waves; 16-bit
-// rows within a wave have twice the arithmetic per byte and want 32 (3 x 409600 of 64: 62 us, 16 waves 72).  Work that does
-// not fill the card once over goes out one step per workgroup.
-int64_t forward_blocks(int64_t groups, int64_t rows, int C, int type) {
-  const RowSplit s = row_split(C, type);
-  const int64_t slots = block_of(s) / s.tpr, want = (rows + slots - 1) / slots;
-  const int64_t full = 2048 * 256 / block_of(s), most = type != MGNN_F32 && s.tpr <= kWave ? full : full / 2;
-  return want * groups <= full ? want : even_blocks(want, groups, most);
+// How many workgroups carry a stream of rows is a matter of bytes in flight: half-empty vectors (a row of 35 floats takes 9
+// of 16 lanes) want twice as many.  `base` full ones, at most what the registers let stand on the card at once.
+int64_t by_bytes(const RowSplit& s, int C, int type, int64_t base, int64_t resident) {
+  const int64_t lanes = (int64_t)s.tpr * s.nv * (16 / elem_bytes(type));
+  return std::min(resident, base * lanes / C);
 }
 
-// Backward: each workgroup leaves one row of shares of dweight and dbias to be added up, so fewer are better as long as
-// two of up to 512 threads stand on every CU (bf16 16384 x 4096, 256 / 512 / 1024 / 2048 workgroups: 106 / 83 / 104 / 115
-// us; fp32 3 x 409600 x 128: 525 / 355 / 369 / 383); and at least four steps each.
+// Forward: workgroups stay, keep their weight rows in registers and load the next row under the sums of this one.  Of 256
+// threads: four per CU for fp32 (3 x 409600 rows of 128, 512 / 1024 / 2048 workgroups: 294 / 229 / 249 us; 958698 of 35, 1024 /
+// 2048: 65 / 54), six for 16-bit rows within a wave, which have twice the arithmetic per byte (3 x 409600 of 64, 1024 / 1536 /
+// 2048: 73 / 61 / 62 us; 958698 of 35: 39 / 33 / 40).  Work that does not fill the card once over goes out one step each.
+int64_t forward_blocks(int64_t groups, int64_t rows, int C, int type) {
+  const RowSplit s = row_split(C, type);
+  const int64_t block = block_of(s), slots = block / s.tpr, want = (rows + slots - 1) / slots;
+  const int64_t most = block > 256 ? 262144 / block : type == MGNN_F32 ? by_bytes(s, C, type, 1024, 2048)
+                                                    : s.nv == 1        ? 1536 : by_bytes(s, C, type, 1024, 1280);
+  return want * groups <= 2048 * 256 / block ? want : even_blocks(want, groups, most);
+}
+
+// Backward: each workgroup leaves one row of shares of dweight and dbias to be added up, so there are fewer, the more so
+// the longer the rows, and each takes at least four steps.  fp32 3 x 409600 x 128, 512 / 768 / 1536 workgroups: 355 / 350 /
+// 383 us; bf16 3 x 409600 x 64: 97 / 92 / 96; 16384 x 4096: 83 / 93 / 107; 8192 columns (512 threads), 256 / 512: 56 / 67; half-
+// empty fp32 958698 x 35, 512 / 1024 / 1280: 129 / 86 / 81.
 int64_t backward_blocks(int64_t groups, int64_t rows, int C, int type) {
   const RowSplit s = row_split(C, type);
-  const int64_t slots = block_of(s) / s.tpr, want = (rows + slots - 1) / slots;
-  const int64_t most = s.tpr > 512 ? 256 : 512;
+  const int64_t block = block_of(s), slots = block / s.tpr, want = (rows + slots - 1) / slots;
+  const bool half = type != MGNN_F32;      // twice the elements and registers per vector
+  const int64_t resident = s.nv == 1 ? half ? 1024 : 2048 : half ? 768 : 1280;
+  const int64_t most = block > 256 ? 256 : by_bytes(s, C, type, half && s.nv == 1 ? 704 : 512, resident);
   return std::max<int64_t>(1, std::min((want + 3) / 4, even_blocks(want, groups, most)));
 }
 
