@@ -23,6 +23,7 @@ extern "C" {
 #define MGNN_ERR_WORKSPACE 4 /* the workspace is too small, missing or not aligned to 8 bytes */
 #define MGNN_ERR_VALUE 5     /* eps or max_norm negative or NaN, a required pointer missing, the norm's gradient list invalid */
 #define MGNN_ERR_OVERLAP 6   /* a gradient that is written overlaps another one of the same call */
+#define MGNN_ERR_MEMORY 7    /* no host memory for the list's tables */
 
 #define MGNN_F32 0
 #define MGNN_BF16 1

@@ -1004,7 +1004,7 @@ int mgnn_grad_norm(const void* const* src, const int64_t* n, const int32_t* type
                    void* workspace, int64_t workspace_bytes, void* stream) try {
   return clip(src, nullptr, n, type, count, groups, -1.0, norms, workspace, workspace_bytes, (hipStream_t)stream);
 } catch (...) {
-  return MGNN_ERR_VALUE;
+  return MGNN_ERR_MEMORY;
 }
 
 int mgnn_clip_grads(const void* const* src, void* const* dst, const int64_t* n, const int32_t* type, int64_t count,
@@ -1012,7 +1012,7 @@ int mgnn_clip_grads(const void* const* src, void* const* dst, const int64_t* n, 
   if (!(max_norm >= 0.0)) return MGNN_ERR_VALUE;
   return clip(src, dst, n, type, count, groups, max_norm, norms, workspace, workspace_bytes, (hipStream_t)stream);
 } catch (...) {
-  return MGNN_ERR_VALUE;
+  return MGNN_ERR_MEMORY;
 }
 
 }  // extern "C"

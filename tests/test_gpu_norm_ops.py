@@ -375,6 +375,72 @@ def test_in_place_clipping_is_seen_by_autograd():
     y.backward()
 
 
+def test_captured_clipping_of_a_long_list():
+  """More tensors than one launch takes, in place: a graph that fills the gradients and clips them, replayed on new values
+  with eager clipping in between."""
+  sizes = [1 + 37 * i for i in range(130)] + [300000]
+  fresh = [normal((n,), i, 0, 0.1) for i, n in enumerate(sizes)]
+  grads = [f.clone() for f in fresh]
+  side = torch.cuda.Stream()
+  side.wait_stream(torch.cuda.current_stream())
+  with torch.cuda.stream(side):
+    norm_ops.clip_grads(grads, 0.5, out=grads)
+  torch.cuda.current_stream().wait_stream(side)
+  graph = torch.cuda.CUDAGraph()
+  with torch.cuda.graph(graph):
+    for g, f in zip(grads, fresh):
+      g.copy_(f)
+    norm = norm_ops.clip_grads(grads, 0.5, out=grads)[1]
+  for k in range(4):
+    for i, f in enumerate(fresh):
+      f.copy_(normal(f.shape, 1000 * k + i, 0, 0.1 + k))
+    want, want_norm = norm_ops.clip_grads(fresh, 0.5)
+    torch.cuda.synchronize()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(norm, want_norm) and all(torch.equal(g, w) for g, w in zip(grads, want)), k
+
+
+def test_two_streams_at_once():
+  """The same operators on two streams without waiting for each other: workspaces are the calls' own."""
+  big = [normal((400000,), 1, 0, 0.1), normal((70000,), 2, 0, 0.1, BF16)]
+  x, w, b, dy = normal((20000, 130), 3), normal((130,), 4), normal((130,), 5), normal((20000, 130), 6)
+  want_clip, want_ln = norm_ops.clip_grads(big, 0.5), both(x, w, b, dy)
+  streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+  torch.cuda.synchronize()
+  got = []
+  for k in range(10):
+    for st in streams:
+      with torch.cuda.stream(st):
+        got.append((norm_ops.clip_grads(big, 0.5), both(x, w, b, dy)))
+  torch.cuda.synchronize()
+  for (out, norm), ln in got:
+    assert torch.equal(norm, want_clip[1]) and all(torch.equal(p, q) for p, q in zip(out, want_clip[0]))
+    assert all(torch.equal(p, q) for p, q in zip(ln, want_ln))
+
+
+def test_offsets_past_32_bits():
+  """Over 2^31 elements, and over 2^32 to the last row of a strided input: the ends of it against calls on the ends alone."""
+  rows, cols = 530000, 4096
+  wide = torch.empty((rows, 2 * cols), dtype=BF16, device='cuda').normal_(0.2, 1.5, generator=torch.Generator(device='cuda').manual_seed(1))
+  x, w, b = wide[:, 5:5 + cols], normal((cols,), 2, 1, 0.2), normal((cols,), 3)
+  dy = torch.ones((rows, cols), dtype=BF16, device='cuda')
+  y, dx, dw, db = both(x, w, b, dy)
+  for part in (slice(0, 3), slice(262143, 262146), slice(rows - 3, rows)):      # the middle one crosses 2^31 elements of the input
+    py, pdx, _, _ = both(x[part], w, b, dy[part])
+    assert torch.equal(y[part], py) and torch.equal(dx[part], pdx)
+  # every partial sum of ones is a whole number below 2^24
+  assert torch.equal(db, torch.full_like(db, float(rows))) and torch.isfinite(dw).all()
+  del wide, x, dy, y, dx
+  n = 2 ** 31 + 77
+  g = torch.full((n,), 0.25, dtype=BF16, device='cuda')
+  norm = norm_ops.clip_grads([g], 1.0, out=[g])[1]
+  want = 0.25 * n ** 0.5
+  assert abs(float(norm) / want - 1) < 2 * U
+  value = torch.tensor(0.25 / (want + 1e-6)).to(BF16)      # the same on every element; one step of the type at most from here
+  assert bool((g == g[0]).all()) and abs(float(g[0]) / float(value) - 1) <= torch.finfo(BF16).eps
+
+
 # ---- together, as an update uses them ----
 
 def _net(layer_norm=True):
@@ -464,6 +530,8 @@ def test_training_with_layer_norm_runs_and_clips():
   before = ctl.policy.norm1_w.detach().clone()
   losses = ctl.update(ctl.rollout(20))
   assert all(x == x for x in losses) and not torch.equal(before, ctl.policy.norm1_w)
+  ctl.amp = BF16      # autocast: 16-bit activations under the norms, fp32 weights
+  assert all(x == x for x in ctl.update(ctl.rollout(20)))
   env.close()
 
 
