@@ -121,6 +121,29 @@ def test_rows_far_off_centre_and_rows_of_one_value():
   assert torch.isnan(zero).all()
 
 
+def test_tiny_deviations_without_eps():
+  """eps = 0 and deviations of 1e-18, whose squares are ordinary fp32 numbers; and of 1e-20, whose squares (1e-40) come in
+  steps of 2^-149: off by 7e-6 each, half of that in the root, below 1e-4 with all roundings."""
+  for scale, off in ((1e-18, 0.0), (1e-20, 1e-4)):
+    x = normal((1, 7, 300), 1) * scale
+    w, b, dy = torch.ones(1, 300, device='cuda'), torch.zeros(1, 300, device='cuda'), normal((1, 7, 300), 2)
+    want, bound = formula(x, w.unsqueeze(1), b.unsqueeze(1), dy, 0.0)
+    got = both(x[0], w[0], b[0], dy[0], 0.0)
+    for g, r, t in zip(got, want, bound):
+      assert ((g.double() - r[0]).abs() <= t[0] + half_step(r[0].abs() + t[0], F32) + off * r[0].abs().max()).all()
+
+
+def test_the_largest_number_of_agents():
+  n = norm_ops.MAX_GROUPS
+  x, w, b, dy = normal((n, 2, 5), 1), normal((n, 5), 2, 1, 0.2), normal((n, 5), 3), normal((n, 2, 5), 4)
+  want, bound = formula(x, w.unsqueeze(1), b.unsqueeze(1), dy, 1e-5)
+  compare(both(x, w, b, dy), want, bound, (F32,) * 4)
+  with pytest.raises(ValueError):
+    norm_ops.layer_norm(torch.zeros(n + 1, 2, device='cuda'), torch.zeros(n + 1, 2, device='cuda'))
+  check_clip([normal((n, 3), 5), normal((n,), 6)], 0.5, stacked=n)
+  check_clip([normal((n, 3), i) for i in range(113)], 0.5, stacked=n)
+
+
 def test_nan_and_infinity_stay_in_their_row():
   x = normal((6, 777), 1)
   x[1, 5], x[3, 776], x[4, 0] = float('nan'), float('inf'), float('-inf')
