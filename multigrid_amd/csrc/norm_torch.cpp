@@ -1,8 +1,8 @@
 // The torch side of include/mgrid_norm.h: argument checks, autograd and memory of layer_norm, grad_norm and clip_grads, with
 // the plain torch expression of the same formulas for tensors that are not on a GPU.  multigrid_amd/norm_ops.py documents and
 // re-exports them.  In C++ because the smallest calls are bound by their host time: the autograd graph's nodes, the
-// allocations and a list of gradients cost several times as much from Python (forward and backward of a small layer norm
-// 98 us from Python; a list of 36 gradients 47 us).
+// allocations and a list of gradients cost several times as much from Python (a small layer norm's forward call 9.4 us
+// against 4.2 here, forward and backward 98 against 61, clipping a list of 36 gradients 48 against 14).
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
