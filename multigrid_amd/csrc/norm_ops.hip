@@ -553,10 +553,11 @@ constexpr int kChunkBytes = kBlock * 16 * 4;
 struct GradTable {
   const void* src[kTensors];
   void* dst[kTensors];
-  int64_t n[kTensors];     // elements per group
-  int32_t end[kTensors];   // chunks of a group up to and with this tensor
-  uint8_t type[kTensors];
+  int64_t n_type[kTensors];      // elements per group << 2 | type (a scalar load takes words)
+  int32_t end[kTensors];         // chunks of a group up to and with this tensor
   int32_t count;
+  __host__ __device__ int64_t n(int i) const { return n_type[i] >> 2; }
+  __host__ __device__ int type(int i) const { return (int)(n_type[i] & 3); }
 };
 static_assert(sizeof(GradTable) <= 3800, "kernel arguments hold 4 KB");
 
@@ -568,15 +569,19 @@ __device__ __forceinline__ double block_sum(double v, double* lds) {      // in 
   return threadIdx.x < kWave ? lanes_sum<BLOCK / kWave>(lds[threadIdx.x % (BLOCK / kWave)]) : 0.0;
 }
 
-__device__ __forceinline__ int find_tensor(const GradTable& t, int chunk) {
-  int lo = 0, hi = t.count - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi) / 2;
-    if (chunk < t.end[mid]) hi = mid;
-    else lo = mid + 1;
+// The tensor of a chunk: the number of tensors that end at or before it, counted by a wave's lanes in one go
+struct Finder {
+  int low, high;      // this lane's two ends
+  __device__ __forceinline__ explicit Finder(const GradTable& t) {
+    const int lane = threadIdx.x % kWave;
+    low = lane < t.count ? t.end[lane] : INT32_MAX;
+    high = lane + kWave < t.count ? t.end[lane + kWave] : INT32_MAX;
   }
-  return lo;
-}
+  __device__ __forceinline__ int operator()(int chunk) const {
+    return __popcll(__ballot(low <= chunk)) + __popcll(__ballot(high <= chunk));
+  }
+};
+static_assert(kTensors <= 2 * kWave);
 
 // Squares are exact in fp64, and no fp32 value overflows there; the conversions hide under the loads: 2.1 GB of fp32 in
 // 337 us (6.4 TB/s), which is all that bounds it.
@@ -599,14 +604,15 @@ __device__ __forceinline__ double chunk_squares(const T* p, int64_t n) {      //
 __global__ __launch_bounds__(kBlock, 8) void grad_squares_kernel(GradTable t, double* partial, int row, int rows_of_group) {
   __shared__ double lds[kBlock / kWave];
   const int64_t g = blockIdx.y;
+  const Finder find(t);
   const int chunks = t.end[t.count - 1];
   double acc = 0.0;
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
-    const int i = find_tensor(t, c);
-    const int64_t at = (int64_t)(c - (i ? t.end[i - 1] : 0)) * (kChunkBytes / (t.type[i] == MGNN_F32 ? 4 : 2));
-    const int64_t off = g * t.n[i] + at, n = t.n[i] - at;
-    if (t.type[i] == MGNN_F32) acc += chunk_squares(static_cast<const float*>(t.src[i]) + off, n);
-    else if (t.type[i] == MGNN_BF16) acc += chunk_squares(static_cast<const __bf16*>(t.src[i]) + off, n);
+    const int i = __builtin_amdgcn_readfirstlane(find(c));
+    const int64_t at = (int64_t)(c - (i ? t.end[i - 1] : 0)) * (kChunkBytes / (t.type(i) == MGNN_F32 ? 4 : 2));
+    const int64_t off = g * t.n(i) + at, n = t.n(i) - at;
+    if (t.type(i) == MGNN_F32) acc += chunk_squares(static_cast<const float*>(t.src[i]) + off, n);
+    else if (t.type(i) == MGNN_BF16) acc += chunk_squares(static_cast<const __bf16*>(t.src[i]) + off, n);
     else acc += chunk_squares(static_cast<const _Float16*>(t.src[i]) + off, n);
   }
   acc = block_sum<kBlock>(acc, lds);
@@ -660,17 +666,18 @@ __global__ __launch_bounds__(kBlock, 8) void grad_scale_kernel(GradTable t, cons
   __shared__ double lds[kBlock / kWave];
   __shared__ float factor;
   const int64_t g = blockIdx.y;
+  const Finder find(t);
   const double norm = group_norm(partial, g, rows_of_group, lds);
   const float f = clip_factor(norm, max_norm, &factor);
   if (norms && blockIdx.x == 0 && threadIdx.x == 0) norms[g] = (float)norm;
   // from the end on, which was read last: what the caches still hold of it is not read from memory again
   for (int c = t.end[t.count - 1] - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {
-    const int i = find_tensor(t, c);
+    const int i = __builtin_amdgcn_readfirstlane(find(c));
     if (f == 1.f && t.src[i] == t.dst[i]) continue;      // a factor of 1 in place: nothing changes
-    const int64_t at = (int64_t)(c - (i ? t.end[i - 1] : 0)) * (kChunkBytes / (t.type[i] == MGNN_F32 ? 4 : 2));
-    const int64_t off = g * t.n[i] + at, n = t.n[i] - at;
-    if (t.type[i] == MGNN_F32) chunk_scale(static_cast<const float*>(t.src[i]) + off, static_cast<float*>(t.dst[i]) + off, n, f, past_caches);
-    else if (t.type[i] == MGNN_BF16)
+    const int64_t at = (int64_t)(c - (i ? t.end[i - 1] : 0)) * (kChunkBytes / (t.type(i) == MGNN_F32 ? 4 : 2));
+    const int64_t off = g * t.n(i) + at, n = t.n(i) - at;
+    if (t.type(i) == MGNN_F32) chunk_scale(static_cast<const float*>(t.src[i]) + off, static_cast<float*>(t.dst[i]) + off, n, f, past_caches);
+    else if (t.type(i) == MGNN_BF16)
       chunk_scale(static_cast<const __bf16*>(t.src[i]) + off, static_cast<__bf16*>(t.dst[i]) + off, n, f, past_caches);
     else chunk_scale(static_cast<const _Float16*>(t.src[i]) + off, static_cast<_Float16*>(t.dst[i]) + off, n, f, past_caches);
   }
@@ -740,12 +747,12 @@ __global__ __launch_bounds__(kSmallBlock) void grad_small_kernel(GradTable t, do
   if (threadIdx.x >= t.count && threadIdx.x < 2 * kSearch - 1) end[threadIdx.x] = INT32_MAX;
   if (threadIdx.x < t.count) {
     const int i = threadIdx.x;
-    const int64_t off = g * t.n[i] * (t.type[i] == MGNN_F32 ? 4 : 2);
+    const int64_t off = g * t.n(i) * (t.type(i) == MGNN_F32 ? 4 : 2);
     end[i] = t.end[i];
     from[i] = static_cast<const char*>(t.src[i]) + off;
     to[i] = t.dst[i] ? static_cast<char*>(t.dst[i]) + off : nullptr;
-    len[i] = (int32_t)t.n[i];
-    type[i] = t.type[i];
+    len[i] = (int32_t)t.n(i);
+    type[i] = t.type(i);
   }
   __syncthreads();
   const int vectors = end[t.count - 1];
@@ -847,22 +854,21 @@ int grad_plan(const void* const* src, void* const* dst, const int64_t* n, const 
     chunks += c;
     t.src[t.count] = src ? src[i] : nullptr;
     t.dst[t.count] = dst ? dst[i] : nullptr;
-    t.n[t.count] = n[i];
-    t.type[t.count] = (uint8_t)type[i];
+    t.n_type[t.count] = n[i] << 2 | type[i];
     t.end[t.count++] = (int32_t)chunks;
   }
   if (plan.tables.size() == 1) {
     GradTable& t = plan.tables[0];
     int64_t vectors = 0;
     for (int i = 0; i < t.count; ++i) {
-      const int V = t.type[i] == MGNN_F32 ? 4 : 8;
-      vectors += t.n[i] / V + (t.n[i] % V != 0);
+      const int V = t.type(i) == MGNN_F32 ? 4 : 8;
+      vectors += t.n(i) / V + (t.n(i) % V != 0);
       if (vectors > kSmallSlots * kSmallBlock) break;
     }
     if (vectors <= kSmallSlots * kSmallBlock) {
       for (int i = 0, v = 0; i < t.count; ++i) {
-        const int V = t.type[i] == MGNN_F32 ? 4 : 8;
-        t.end[i] = v += (int)((t.n[i] + V - 1) / V);
+        const int V = t.type(i) == MGNN_F32 ? 4 : 8;
+        t.end[i] = v += (int)((t.n(i) + V - 1) / V);
       }
       plan.slots = (int)((vectors + 4 * kSmallBlock - 1) / (4 * kSmallBlock)) * 4;
       return MGNN_OK;
@@ -915,7 +921,7 @@ int clip(const void* const* src, void* const* dst, const int64_t* n, const int32
   if (dst && overlaps(src, dst, n, type, count, groups)) return MGNN_ERR_OVERLAP;
   if (plan.slots) {
     const GradTable& t = plan.tables[0];
-    const bool floats = std::all_of(t.type, t.type + t.count, [](uint8_t ty) { return ty == MGNN_F32; });
+    const bool floats = std::all_of(t.n_type, t.n_type + t.count, [](int64_t nt) { return (nt & 3) == MGNN_F32; });
     const auto pick = [&](auto all) {
       constexpr bool F = decltype(all)::value;
       return plan.slots == 4 ? grad_small_kernel<4, F> : plan.slots == 8 ? grad_small_kernel<8, F>

@@ -558,6 +558,16 @@ def test_training_with_layer_norm_runs_and_clips():
   env.close()
 
 
+def test_the_training_command_with_layer_norm(tmp_path, capsys):
+  import json
+  from multigrid_amd import train
+  train.main(['--envs', '256', '--steps', '10', '--iters', '2', '--window', '1', '--layer-norm', '--hang-dump', '0', '--out', str(tmp_path / 'best')])
+  lines = [json.loads(l) for l in capsys.readouterr().out.splitlines() if l.startswith('{')]
+  assert [l['iter'] for l in lines] == [0, 1] and all(x == x for l in lines for x in l['loss'])
+  weights = torch.load(str(tmp_path / 'best_agent_0.pth'), weights_only=True)
+  ppo.AgentNet(layer_norm=True).load_state_dict(weights)
+
+
 def test_per_agent_nets_are_clipped_one_by_one():
   torch.manual_seed(0)
   nets = ppo.PerAgentNets([ppo.MultiGridPPONet(n_agents=2) for _ in range(2)], all_dirs=True).cuda()
