@@ -686,12 +686,15 @@ __global__ __launch_bounds__(kBlock, 8) void grad_scale_kernel(GradTable t, cons
 // Norms and clipping of gradients that one workgroup per group holds in its registers, SLOTS vectors of 16 bytes a thread:
 // one launch, and every element is read once.  The list's vectors are numbered through (t.end: vectors up to and with a
 // tensor); a tensor's last vector ends at its end and overlaps the one before, which counts the common elements; both
-// write the same values.  37544 fp32 in 13 tensors take 8.7 us: setting up and finding the tensors 1.4, loading 1.5, fp64 squares
-// 1.9, the norm 0.6, scaling and storing 2.7, all on one CU; two launches over many CUs take 4.4 + 5.1.  FLOATS: all of the list is fp32.  max_norm < 0: the norms alone.
+// write the same values.  37544 fp32 in 13 tensors take 8.2 us, all on one CU: the table and each vector's tensor 0.9, loading
+// 1.5, fp64 squares 1.9, the norm 0.6, scaling and storing 2.7; two launches over many CUs take 4.4 + 5.1.  FLOATS: all of the
+// list is fp32.  max_norm < 0: the norms alone.
 constexpr int kSmallBlock = 1024;
-constexpr int kSearch = 64;          // the largest power of two up to kTensors
-static_assert(kSearch <= kTensors && kTensors < 2 * kSearch && kTensors <= kSmallBlock);
 constexpr int kSmallSlots = 16;      // at most: 64 of the 128 registers a thread of 1024 has
+struct SmallTable : GradTable {
+  uint8_t first[kSmallSlots * kSmallBlock / kWave];      // the tensor of every wave's first vector; count past the last one
+};
+static_assert(sizeof(SmallTable) <= 3800 && kTensors < 256 && kTensors < kSmallBlock);
 template <typename T>
 __device__ __forceinline__ double raw_squares(uint4 raw, int skip, int n) {      // elements skip .. n-1 of the vector
   constexpr int V = Pack<T>::V;
@@ -734,44 +737,37 @@ __device__ __forceinline__ void raw_scale(T* p, uint4 raw, int n, float f) {
 }
 
 template <int SLOTS, bool FLOATS>
-__global__ __launch_bounds__(kSmallBlock) void grad_small_kernel(GradTable t, double max_norm, float* norms) {
+__global__ __launch_bounds__(kSmallBlock) void grad_small_kernel(SmallTable t, double max_norm, float* norms) {
   __shared__ double lds[kSmallBlock / kWave];
-  __shared__ int32_t end[2 * kSearch - 1];
+  __shared__ int32_t end[kTensors + 1];
   __shared__ const char* from[kTensors];
   __shared__ char* to[kTensors];
   __shared__ int32_t len[kTensors];
-  __shared__ uint8_t type[kTensors], first[SLOTS * kSmallBlock / kWave];
+  __shared__ uint8_t type[kTensors];
   __shared__ float factor;
   const auto type_of = [&](int i) { return FLOATS ? MGNN_F32 : (int)type[i]; };
   const int64_t g = blockIdx.x;
-  if (threadIdx.x >= t.count && threadIdx.x < 2 * kSearch - 1) end[threadIdx.x] = INT32_MAX;
-  if (threadIdx.x < t.count) {
+  int which[SLOTS], stop[SLOTS];      // each vector's tensor, and where that ends
+#pragma unroll
+  for (int k = 0; k < SLOTS; ++k) which[k] = t.first[k * (kSmallBlock / kWave) + threadIdx.x / kWave];
+  if (threadIdx.x <= t.count) {
     const int i = threadIdx.x;
-    const int64_t off = g * t.n(i) * (t.type(i) == MGNN_F32 ? 4 : 2);
-    end[i] = t.end[i];
-    from[i] = static_cast<const char*>(t.src[i]) + off;
-    to[i] = t.dst[i] ? static_cast<char*>(t.dst[i]) + off : nullptr;
-    len[i] = (int32_t)t.n(i);
-    type[i] = t.type(i);
+    end[i] = i < t.count ? t.end[i] : INT32_MAX;
+    if (i < t.count) {
+      const int64_t off = g * t.n(i) * (t.type(i) == MGNN_F32 ? 4 : 2);
+      from[i] = static_cast<const char*>(t.src[i]) + off;
+      to[i] = t.dst[i] ? static_cast<char*>(t.dst[i]) + off : nullptr;
+      len[i] = (int32_t)t.n(i);
+      type[i] = t.type(i);
+    }
   }
   __syncthreads();
   const int vectors = end[t.count - 1];
-  // the tensor of every wave's first vector: the number of tensors that end at or before it
-  if (threadIdx.x < SLOTS * kSmallBlock / kWave) {
-    int i = 0;
-    for (int half = kSearch; half >= 1; half >>= 1)      // i + half <= 2 * kSearch - 1, the list's last entry
-      if (half <= t.count && end[i + half - 1] <= (int)threadIdx.x * kWave) i += half;
-    first[threadIdx.x] = (uint8_t)i;
-  }
-  __syncthreads();
-  int which[SLOTS], stop[SLOTS];
-#pragma unroll
-  for (int k = 0; k < SLOTS; ++k) which[k] = first[k * (kSmallBlock / kWave) + threadIdx.x / kWave];
 #pragma unroll
   for (int k = 0; k < SLOTS; ++k) stop[k] = end[which[k]];
 #pragma unroll
   for (int k = 0; k < SLOTS; ++k)
-    while (k * kSmallBlock + (int)threadIdx.x >= stop[k]) stop[k] = end[++which[k]];      // ends at a padding entry at the latest
+    while (k * kSmallBlock + (int)threadIdx.x >= stop[k]) stop[k] = end[++which[k]];      // end[count], at the latest, is past them all
   uint4 raw[SLOTS];
   int place[SLOTS];      // tensor << 20 | first element; -1: no vector
   static_assert(kSmallSlots * kSmallBlock * 8 <= 1 << 20 && kTensors < 1 << 11);
@@ -920,7 +916,12 @@ int clip(const void* const* src, void* const* dst, const int64_t* n, const int32
   }
   if (dst && overlaps(src, dst, n, type, count, groups)) return MGNN_ERR_OVERLAP;
   if (plan.slots) {
-    const GradTable& t = plan.tables[0];
+    SmallTable t;
+    static_cast<GradTable&>(t) = plan.tables[0];
+    for (int wave = 0, i = 0; wave < plan.slots * kSmallBlock / kWave; ++wave) {
+      while (i < t.count && t.end[i] <= wave * kWave) ++i;
+      t.first[wave] = (uint8_t)i;
+    }
     const bool floats = std::all_of(t.n_type, t.n_type + t.count, [](int64_t nt) { return (nt & 3) == MGNN_F32; });
     const auto pick = [&](auto all) {
       constexpr bool F = decltype(all)::value;
