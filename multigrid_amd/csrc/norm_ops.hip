@@ -224,8 +224,8 @@ __device__ __forceinline__ void row_stats(const float (&v)[NV * Pack<T>::V], con
   }
 }
 
-// y = (x - m) s w + b.  Bound by HBM, each element read once and written once: 3 x 409600 rows of 128 fp32 218 us (5.8 TB/s),
-// 16384 of 4096 bf16 45 us (5.9); at 3 x 4096 rows of 128 fp32 4.3 us, a launch and one trip to memory.
+// y = (x - m) s w + b.  Bound by HBM, each element read once and written once: 3 x 409600 rows of 128 fp32 219 us (5.7 TB/s),
+// 16384 of 4096 bf16 45 us (5.9); at 3 x 4096 rows of 128 fp32 4.2 us, a launch and one trip to memory.
 template <typename T, int TPR, int NV, bool FULL>
 __global__ __launch_bounds__(Shape<TPR>::BLOCK) void ln_fwd_kernel(const T* x, int64_t ld, const void* weight, const void* bias,
                                                                    int wtype, T* y, float2* stats, int64_t rows, int C, float eps) {
@@ -295,7 +295,7 @@ __device__ __forceinline__ void slots_sum(float (&acc)[NE], float* lds) {
 }
 
 // dx = s (e - mean(e) - h mean(e h)) with e = dy w, and the sums of dy h and dy over this workgroup's rows.  Bound by HBM, x
-// and dy read once, dx written once: 3 x 409600 rows of 128 fp32 363 us (5.2 TB/s), 16384 of 4096 bf16 86 us (4.7); 509 rows
+// and dy read once, dx written once: 3 x 409600 rows of 128 fp32 366 us (5.2 TB/s), 16384 of 4096 bf16 86 us (4.7); 509 rows
 // of 16381 fp32, two to a workgroup, 31 us, a quarter of the traffic shares.
 // partial: [groups][blocks][2][C] floats (this workgroup's shares of dweight and dbias), or NULL with one block per group:
 // then dweight / dbias are written here
@@ -584,7 +584,7 @@ struct Finder {
 static_assert(kTensors <= 2 * kWave);
 
 // Squares are exact in fp64, and no fp32 value overflows there; the conversions hide under the loads: 2.1 GB of fp32 in
-// 337 us (6.4 TB/s), which is all that bounds it.
+// 335 us (6.4 TB/s), which is all that bounds it.
 template <typename T>
 __device__ __forceinline__ double chunk_squares(const T* p, int64_t n) {      // n elements from p on, one chunk at most
   constexpr int V = Pack<T>::V;
@@ -660,7 +660,7 @@ __device__ __forceinline__ void chunk_scale(const T* p, T* q, int64_t n, float f
 }
 
 // Every workgroup adds up the partial sums itself (16 KB at most, from the caches) rather than waiting for a launch between.
-// 2.1 GB of fp32 read and written in 776 us (5.5 TB/s), bound by HBM.
+// 2.1 GB of fp32 read and written in 767 us (5.6 TB/s), bound by HBM.
 __global__ __launch_bounds__(kBlock, 8) void grad_scale_kernel(GradTable t, const double* partial, int rows_of_group, double max_norm,
                                                             float* norms, bool past_caches) {
   __shared__ double lds[kBlock / kWave];
