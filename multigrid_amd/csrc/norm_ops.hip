@@ -637,6 +637,17 @@ __device__ __forceinline__ float clip_factor(double norm, double max_norm, float
   return *lds;
 }
 
+// Lists of many launches leave more partial sums than every workgroup should add up by itself: each group's become one
+constexpr int kMostRows = 16384;      // 128 KB from the caches, 2 us of a scaling launch
+__global__ __launch_bounds__(1024) void grad_sum_kernel(const double* partial, int rows_of_group, double* sums) {
+  __shared__ double lds[1024 / kWave];
+  double acc = 0.0;
+#pragma unroll 8
+  for (int k = threadIdx.x; k < rows_of_group; k += 1024) acc += partial[(int64_t)blockIdx.x * rows_of_group + k];
+  acc = block_sum<1024>(acc, lds);
+  if (threadIdx.x == 0) sums[blockIdx.x] = acc;
+}
+
 __global__ __launch_bounds__(kBlock) void grad_norm_kernel(const double* partial, int rows_of_group, float* norms) {
   __shared__ double lds[kBlock / kWave];
   const double norm = group_norm(partial, blockIdx.x, rows_of_group, lds);
@@ -819,6 +830,7 @@ struct GradPlan {
   std::vector<int> blocks;
   int rows = 0;      // partial sums per group; 0 with a table: one workgroup per group does it all
   int slots = 0;     // then its vectors per thread
+  int64_t workspace(int64_t groups) const { return (rows + (rows > kMostRows)) * groups * (int64_t)sizeof(double); }
 };
 
 // chunks a tensor is cut into; -1: not a tensor that the list may hold
@@ -932,7 +944,7 @@ int clip(const void* const* src, void* const* dst, const int64_t* n, const int32
     hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kSmallBlock), 0, stream, t, dst ? max_norm : -1.0, norms);
     return launched();
   }
-  if (!workspace || (uintptr_t)workspace % 8 || workspace_bytes < plan.rows * groups * (int64_t)sizeof(double)) return MGNN_ERR_WORKSPACE;
+  if (!workspace || (uintptr_t)workspace % 8 || workspace_bytes < plan.workspace(groups)) return MGNN_ERR_WORKSPACE;
   double* partial = static_cast<double*>(workspace);
   int row = 0;
   for (size_t k = 0; k < plan.tables.size(); ++k) {
@@ -940,8 +952,15 @@ int clip(const void* const* src, void* const* dst, const int64_t* n, const int32
                        plan.rows);
     row += plan.blocks[k];
   }
+  int rows = plan.rows;
+  if (rows > kMostRows) {
+    double* sums = partial + rows * groups;
+    hipLaunchKernelGGL(grad_sum_kernel, dim3((unsigned)groups), dim3(1024), 0, stream, partial, rows, sums);
+    partial = sums;
+    rows = 1;
+  }
   if (!dst) {
-    hipLaunchKernelGGL(grad_norm_kernel, dim3((unsigned)groups), dim3(kBlock), 0, stream, partial, plan.rows, norms);
+    hipLaunchKernelGGL(grad_norm_kernel, dim3((unsigned)groups), dim3(kBlock), 0, stream, partial, rows, norms);
     return launched();
   }
   // Results of more than the 256 MB of the memory-side cache go past it: they would push out the gradients that are still
@@ -952,7 +971,7 @@ int clip(const void* const* src, void* const* dst, const int64_t* n, const int32
   const bool past_caches = bytes >= (int64_t)256 << 20;
   for (size_t k = plan.tables.size(); k-- > 0;)
     hipLaunchKernelGGL(grad_scale_kernel, dim3(plan.blocks[k], (unsigned)groups), dim3(kBlock), 0, stream, plan.tables[k], partial,
-                       plan.rows, max_norm, k == 0 ? norms : nullptr, past_caches);
+                       rows, max_norm, k == 0 ? norms : nullptr, past_caches);
   return launched();
 }
 
@@ -1014,7 +1033,7 @@ int mgnn_layer_norm_backward(const void* x, int64_t ld, const void* dy, const vo
 int64_t mgnn_grad_norm_workspace(const int64_t* n, const int32_t* type, int64_t count, int64_t groups) try {
   GradPlan plan;
   if (grad_plan(nullptr, nullptr, n, type, count, groups, plan)) return -1;
-  return plan.rows * groups * (int64_t)sizeof(double);
+  return plan.workspace(groups);
 } catch (...) {
   return -1;
 }

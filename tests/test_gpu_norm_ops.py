@@ -314,6 +314,12 @@ def test_clip_a_list_over_all_launch_shapes():
     check_clip([normal((2, n // 2), 3, 0, 0.01, BF16), normal((2, 1), 4)], 0.5, stacked=2)
 
 
+def test_clip_a_list_of_many_large_tensors():
+  """Ten launches of full grids, whose partial sums are joined by a kernel of their own; norm alone, apart and in place."""
+  check_clip([normal((76000 + i,), i, 0, 0.001) for i in range(1120)], 0.5)
+  check_clip([normal((2, 76000 + i), i, 0, 0.001, BF16) for i in range(1120)], 0.5, stacked=2)
+
+
 @pytest.mark.parametrize('dtype', [F32, BF16])
 def test_clip_views_of_one_buffer(dtype):
   """Gradients and results as neighbouring parts of flat buffers, none of them aligned."""
