@@ -9,6 +9,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/utils/pybind.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <tuple>
@@ -171,6 +172,117 @@ void check_grads(const Tensors& grads, int64_t stacked) {
   }
 }
 
+// Whether a sum of step * i over all terms, with 0 <= i <= most for each, can be `total`: exactly, by the terms from the largest
+// step down.  Steps that nest, as those of a slice do, leave two or three choices each, and a rest whose terms reach every
+// value needs none; other steps may leave many, of which 2^20 are tried before the answer is yes.
+class Sums {
+ public:
+  void add(int64_t step, int64_t most) {
+    if (step > 0 && most > 0) terms_.push_back({step, most, 0, false});
+  }
+  bool reach(int64_t total) {
+    std::sort(terms_.begin(), terms_.end(), [](const Term& a, const Term& b) { return a.step < b.step; });
+    int64_t below = 0;
+    bool every = true;
+    size_t n = 0;
+    for (const Term& t : terms_) {
+      if (n && terms_[n - 1].step == t.step) terms_[n - 1].most += t.most;
+      else terms_[n++] = t;
+    }
+    terms_.resize(n);
+    for (Term& t : terms_) {
+      t.below = below;
+      t.every = every;
+      every = every && t.step <= below + 1;
+      below += t.step * t.most;
+    }
+    tries_ = 1 << 20;
+    return search(n, total, below, every);
+  }
+
+ private:
+  struct Term {
+    int64_t step, most;
+    int64_t below;      // what the smaller ones reach together
+    bool every;         // whether they reach all values up to that
+  };
+  bool search(size_t n, int64_t total, int64_t limit, bool every) {
+    if (total < 0 || total > limit) return false;
+    if (every) return true;
+    const Term& t = terms_[n - 1];
+    const int64_t high = std::min(t.most, total / t.step), low = std::max<int64_t>(0, (total - t.below + t.step - 1) / t.step);
+    for (int64_t i = high; i >= low; --i)
+      if (--tries_ < 0 || search(n - 1, total - i * t.step, t.below, t.every)) return true;
+    return false;
+  }
+  std::vector<Term> terms_;
+  int64_t tries_ = 0;
+};
+
+// Whether two of t's elements lie at one address: with k the axis of largest number along which their places differ by at least 1, the
+// other differences, counted from the least possible one, have to make up for it
+bool overlaps_itself(const Tensor& t) {
+  if (t.numel() <= 1 || t.is_non_overlapping_and_dense()) return false;
+  for (int64_t k = 0; k < t.dim(); ++k) {
+    if (t.size(k) <= 1) continue;
+    Sums sums;
+    int64_t total = -t.stride(k);
+    for (int64_t d = 0; d < t.dim(); ++d) {
+      sums.add(t.stride(d), d == k ? t.size(d) - 2 : 2 * (t.size(d) - 1));
+      if (d != k) total += t.stride(d) * (t.size(d) - 1);
+    }
+    if (sums.reach(total)) return true;
+  }
+  return false;
+}
+
+// A tensor's elements in memory
+struct Place {
+  const Tensor* t;
+  uintptr_t from, to;      // its first byte, and the one behind its last
+  size_t index;
+  bool written;
+};
+Place place_of(const Tensor& t, size_t index, bool written) {
+  uintptr_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) last += t.stride(d) * (t.size(d) - 1);
+  const uintptr_t from = reinterpret_cast<uintptr_t>(written ? t.mutable_data_ptr() : t.const_data_ptr());
+  return {&t, from, from + (last + 1) * t.element_size(), index, written};
+}
+bool overlap(const Place& a, const Place& b) {      // a.from <= b.from
+  if (b.from >= a.to) return false;
+  Sums sums;
+  int64_t total = b.to - 1 - a.from;      // a's bytes counted from its first, b's from its last backwards
+  for (const Place* p : {&a, &b}) {
+    sums.add(1, p->t->element_size() - 1);
+    for (int64_t d = 0; d < p->t->dim(); ++d) sums.add(p->t->stride(d) * p->t->element_size(), p->t->size(d) - 1);
+  }
+  return sums.reach(total);
+}
+
+// Refuses results whose memory holds another result, another tensor's gradient or two elements of their own.  (A result may
+// lie over its own gradient: that is read whole before the result is written, or is the very same tensor.)
+void check_memory(const Tensors& grads, const Tensors& out) {
+  std::vector<Place> places;
+  for (size_t i = 0; i < out.size(); ++i) {
+    const Tensor &o = out[i], &g = grads[i];
+    // tensors without memory of their own: those of the meta device, and stand-ins for others
+    if (o.numel() == 0 || o.key_set().has(c10::DispatchKey::Meta) || g.key_set().has(c10::DispatchKey::Meta)) continue;
+    TORCH_CHECK_VALUE(!overlaps_itself(o), "a gradient that is written has several elements at one address (it overlaps itself)");
+    places.push_back(place_of(o, i, true));
+    if (!g.is_same(o)) places.push_back(place_of(g, i, false));
+  }
+  std::sort(places.begin(), places.end(), [](const Place& a, const Place& b) { return a.from < b.from; });
+  std::vector<const Place*> open;      // those that may reach the next one
+  for (const Place& p : places) {
+    open.erase(std::remove_if(open.begin(), open.end(), [&](const Place* q) { return q->to <= p.from; }), open.end());
+    for (const Place* q : open)
+      TORCH_CHECK_VALUE(q->index == p.index || !(q->written || p.written) || !overlap(*q, p),
+                        "clip_grads: a gradient that is written overlaps another one of the call");
+    open.push_back(&p);
+  }
+}
+
 std::vector<int64_t> norm_shape(int64_t stacked) { return stacked ? std::vector<int64_t>{stacked} : std::vector<int64_t>{}; }
 
 Tensor plain_norms(const Tensors& grads, int64_t stacked) {      // float64
@@ -229,13 +341,12 @@ std::tuple<Tensors, Tensor> clip_grads(const Tensors& grads, double max_norm, in
       const Tensor &o = out[i], &g = grads[i];
       TORCH_CHECK_VALUE(o.sizes() == g.sizes() && o.scalar_type() == g.scalar_type() && o.device() == g.device() && o.layout() == at::kStrided,
                         "out does not match the gradients in shape, type or device");
-      for (int64_t d = 0; d < o.dim() && !o.is_contiguous(); ++d)
-        TORCH_CHECK_VALUE(o.size(d) <= 1 || o.stride(d) != 0, "a gradient that is written has several elements at one address (an expanded tensor)");
     }
   } else {
     for (const Tensor& g : grads) out.push_back(at::empty_like(g));
   }
   if (count == 0 || !grads[0].is_cuda()) {
+    if (given) check_memory(grads, out);
     const Tensor norms = plain_norms(grads, stacked), factor = (max_norm / (norms + 1e-6)).clamp_max(1.0).to(at::kFloat);
     for (size_t i = 0; i < count; ++i) {
       std::vector<int64_t> wide(grads[i].dim(), 1);
@@ -244,10 +355,14 @@ std::tuple<Tensors, Tensor> clip_grads(const Tensors& grads, double max_norm, in
     }
     return {out, norms.to(at::kFloat)};
   }
-  // tensors without a common dense order go through contiguous copies
+  // tensors without a common dense order go through contiguous copies; the kernels' entry point, which sees those instead of the
+  // caller's memory, checks the lists that need none
   Tensors src(grads), dst(out);
+  bool copies = false;
   for (size_t i = 0; i < count; ++i) {
     if ((src[i].is_contiguous() && dst[i].is_contiguous()) || (src[i].strides() == dst[i].strides() && dense(src[i], stacked))) continue;
+    if (given && !copies) check_memory(grads, out);
+    copies = true;
     src[i] = src[i].contiguous();
     dst[i] = at::empty(out[i].sizes(), out[i].options());
   }

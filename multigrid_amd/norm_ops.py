@@ -55,8 +55,9 @@ def grad_norm(grads, stacked=0):
 
 def clip_grads(grads, max_norm, stacked=0, out=None):
   """([g * min(1, max_norm / (norm + 1e-6)) for every gradient g], norm) with norm = grad_norm(grads, stacked); agent by
-  agent if stacked.  out: tensors of the gradients' shapes and types that receive the results (the gradients themselves:
-  in place); none of them may overlap another gradient of the call.  A norm that is NaN makes every result NaN."""
+  agent if stacked.  out: tensors of the gradients' shapes and types that receive the results, each its gradient itself (in
+  place) or other memory; none of them may overlap itself, another result or another gradient of the call.  A norm that is
+  NaN makes every result NaN."""
   return (_EXT or load()).clip_grads([grads] if isinstance(grads, torch.Tensor) else list(grads), max_norm, stacked,
                                      out if out is None else list(out))
 

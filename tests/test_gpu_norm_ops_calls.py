@@ -1,0 +1,40 @@
+"""Calls of multigrid_amd/norm_ops.py on the GPU that must be refused, or that must return what simpler calls return."""
+import pytest
+import torch
+
+from multigrid_amd import norm_ops
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+
+
+def normal(shape, seed, mean=0.0, std=1.0, dtype=torch.float32):
+  g = torch.Generator(device='cuda').manual_seed(seed)
+  return torch.empty(shape, device='cuda').normal_(mean, std, generator=g).to(dtype)
+
+
+def test_clipping_refuses_strided_memory_that_it_would_write_twice():
+  """Tensors that go through contiguous copies: their own memory counts, and nothing is written before the refusal."""
+  w, q = normal((8, 10), 1), normal((40,), 2)
+  for grads, out in (([normal((8, 5), 3), normal((8, 5), 4)], [w[:, :5], w[:, 3:8]]),
+                     ([normal((8, 5), 3), w[:, 4:7]], [w[:, :5], torch.zeros(8, 3, device='cuda')]),
+                     ([w[::2], w[4:6]], [w[::2], w[4:6]]),
+                     ([normal((3, 3), 5)], [q.as_strided((3, 3), (1, 1))]),
+                     ([normal((3, 3), 5)], [q.as_strided((3, 3), (2, 1))]),
+                     ([normal((4, 2), 5)], [q[:4, None].expand(4, 2)])):
+    kept = [t.clone() for t in grads + out]
+    with pytest.raises(ValueError, match='overlap'):
+      norm_ops.clip_grads(grads, 0.5, out=out)
+    assert all(torch.equal(t, k) for t, k in zip(grads + out, kept))
+
+
+def test_clipping_takes_strided_neighbours():
+  w, q = normal((8, 10), 1), normal((24,), 2)
+  for parts in ([w[:, :5], w[:, 5:]], [w[::2], w[1::2]], [q[0::3], q[1::3], q[2::3]], [w[:4, :3], w[:4, 3:9], w[4:, 1:]], [w[:, :0], w]):
+    norm = torch.sqrt(sum(p.double().square().sum() for p in parts))
+    want = [p.double() * torch.clamp(0.5 / (norm + 1e-6), max=1.0) for p in parts]
+    got = norm_ops.clip_grads(parts, 0.5, out=parts)[1]
+    assert abs(float(got) - float(norm)) <= float(norm) * U * 1.01
+    # the factor's two roundings and the product's
+    assert all(((p.double() - v).abs() <= v.abs() * (4 * U)).all() for p, v in zip(parts, want))
