@@ -39,6 +39,11 @@ void check(int rc, const char* what) {
   TORCH_CHECK_VALUE(rc == MGNN_OK, what, ": refused with MGNN error ", rc);
 }
 
+// The kernels carry no forward-mode tangent, and would lose that of an input without a word
+void check_no_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative on a GPU");
+}
+
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
 
 Tensor bytes_on(const Tensor& t, int64_t size) { return size > 0 ? at::empty({size}, t.options().dtype(at::kByte)) : Tensor(); }
@@ -84,6 +89,7 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "layer_norm is differentiable once: its gradients have no graph (create_graph)");
+    check_no_tangent(grads[0], "layer_norm's backward pass");
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &stats = saved[1], &w = saved[2];
     const int64_t ld = ctx->saved_data["ld"].toInt();
@@ -144,6 +150,9 @@ Tensor layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor&
                     "layer_norm's weight and bias differ in shape or type");
   TORCH_CHECK_VALUE(s.groups <= MGNN_MAX_GROUPS, "layer_norm takes at most ", MGNN_MAX_GROUPS, " weight rows, not ", s.groups);
   if (!x.is_cuda()) return plain_layer_norm(x, weight, bias, eps);
+  check_no_tangent(x, "layer_norm");
+  if (weight) check_no_tangent(*weight, "layer_norm");
+  if (bias) check_no_tangent(*bias, "layer_norm");
   s.rows = s.groups ? x.numel() / s.cols / s.groups : 0;
   const c10::DeviceGuard guard(x.device());
   if (at::GradMode::is_enabled() && (x.requires_grad() || (weight && weight->requires_grad()) || (bias && bias->requires_grad())))
@@ -323,6 +332,7 @@ Tensor grad_norm(const Tensors& grads, int64_t stacked) {
   const at::NoGradGuard no_grad;
   check_grads(grads, stacked);
   if (grads.empty() || !grads[0].is_cuda()) return plain_norms(grads, stacked).to(at::kFloat);
+  for (const Tensor& g : grads) check_no_tangent(g, "grad_norm");
   Tensors src;
   for (const Tensor& g : grads) src.push_back(dense(g, stacked) ? g : g.contiguous());
   return launch(src, nullptr, 0.0, stacked);
@@ -355,6 +365,7 @@ std::tuple<Tensors, Tensor> clip_grads(const Tensors& grads, double max_norm, in
     }
     return {out, norms.to(at::kFloat)};
   }
+  for (const Tensor& g : grads) check_no_tangent(g, "clip_grads");
   // tensors without a common dense order go through contiguous copies; the kernels' entry point, which sees those instead of the
   // caller's memory, checks the lists that need none
   Tensors src(grads), dst(out);

@@ -6,7 +6,8 @@ epoch (v8_robust_ppo.py:340).  `clip_grads` is the same clipping into other tens
 they run the HIP kernels of libmgnn.so on the current stream, for float32, bfloat16 and float16; other tensors take the
 plain torch expression of the same formulas.  The checks, the autograd node and the memory are csrc/norm_torch.cpp, built as
 _norm_ops.so; a missing library raises.  What is not taken is refused with a TypeError (types, layouts) or a ValueError
-(shapes, sizes, devices, overlapping memory) before anything is written.
+(shapes, sizes, devices, overlapping memory) before anything is written; what would lose its derivative, with a RuntimeError
+(NotImplementedError for forward-mode tangents, which the kernels do not carry).
 
 Nothing is kept between calls: workspaces come from torch's allocator, so every captured graph has its own.  As with any
 torch operator, a backward pass that is captured needs leaves whose eager graphs are gone.
@@ -43,7 +44,7 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
   """Layer norm over the last axis: (x - mean) / sqrt(mean((x - mean)^2) + eps) * weight + bias, in x's type, with the
   statistics and every sum in float32.  weight / bias: [cols] of x's type or float32, or None; [x.shape[0], cols] gives
   every index of x's leading axis (an agent) its own.  Rows of 1 to 16384 elements.  Differentiable in all three, once: on
-  a GPU its gradients have no graph, and asking for one (create_graph) raises."""
+  a GPU its gradients have no graph, and asking for one (create_graph) raises, as a forward-mode tangent does."""
   return (_EXT or load()).layer_norm(x, weight, bias, eps)
 
 

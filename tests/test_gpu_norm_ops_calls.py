@@ -38,3 +38,25 @@ def test_clipping_takes_strided_neighbours():
     assert abs(float(got) - float(norm)) <= float(norm) * U * 1.01
     # the factor's two roundings and the product's
     assert all(((p.double() - v).abs() <= v.abs() * (4 * U)).all() for p, v in zip(parts, want))
+
+
+def test_forward_derivatives_are_refused():
+  """The kernels carry no tangents: a dual input, or a dual gradient in the backward pass, raises instead of losing its own."""
+  from torch.autograd import forward_ad
+  x, w, b = normal((6, 20), 1), normal((20,), 2), normal((20,), 3)
+  with forward_ad.dual_level():
+    dual = [forward_ad.make_dual(t, torch.ones_like(t)) for t in (x, w, b)]
+    for args in ((dual[0], w, b), (x, dual[1], b), (x, w, dual[2]), (x, None, dual[2]), (dual[0].t().contiguous().t(), w, b)):
+      with pytest.raises(NotImplementedError, match='forward'):
+        norm_ops.layer_norm(*args)
+    with pytest.raises(NotImplementedError, match='forward'):
+      norm_ops.grad_norm([x, dual[0]])
+    with pytest.raises(NotImplementedError, match='forward'):
+      norm_ops.clip_grads([x, dual[0]], 0.5)
+    wg = w.clone().requires_grad_(True)
+    y = norm_ops.layer_norm(x, wg, b)
+    with pytest.raises(NotImplementedError, match='forward'):
+      torch.autograd.grad(y, wg, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+    y = norm_ops.layer_norm(x, w, b)      # plain tensors in the same level
+    assert forward_ad.unpack_dual(y).tangent is None
+  assert torch.equal(norm_ops.layer_norm(x, w, b), y)
