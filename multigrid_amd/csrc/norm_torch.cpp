@@ -5,8 +5,10 @@
 // against 4.2 here, forward and backward 98 against 61, clipping a list of 36 gradients 48 against 14).
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include <algorithm>
@@ -42,6 +44,14 @@ void check(int rc, const char* what) {
 // The kernels carry no forward-mode tangent, and would lose that of an input without a word
 void check_no_tangent(const Tensor& t, const char* what) {
   TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), what, " has no forward-mode derivative on a GPU");
+}
+
+// A trace (torch.jit.trace, make_fx) records the allocation of a kernel's results but not the kernel: its replay would return
+// memory that nothing has written
+void check_no_trace(const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() &&
+                                  !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY),
+                              what, "'s kernels cannot be recorded in a trace");
 }
 
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
@@ -90,6 +100,7 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, const torch::autograd::variable_list& grads) {
     TORCH_CHECK(!at::GradMode::is_enabled(), "layer_norm is differentiable once: its gradients have no graph (create_graph)");
     check_no_tangent(grads[0], "layer_norm's backward pass");
+    check_no_trace("layer_norm's backward pass");
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &stats = saved[1], &w = saved[2];
     const int64_t ld = ctx->saved_data["ld"].toInt();
@@ -150,6 +161,7 @@ Tensor layer_norm(const Tensor& x, const MaybeTensor& weight, const MaybeTensor&
                     "layer_norm's weight and bias differ in shape or type");
   TORCH_CHECK_VALUE(s.groups <= MGNN_MAX_GROUPS, "layer_norm takes at most ", MGNN_MAX_GROUPS, " weight rows, not ", s.groups);
   if (!x.is_cuda()) return plain_layer_norm(x, weight, bias, eps);
+  check_no_trace("layer_norm");
   check_no_tangent(x, "layer_norm");
   if (weight) check_no_tangent(*weight, "layer_norm");
   if (bias) check_no_tangent(*bias, "layer_norm");
@@ -332,6 +344,7 @@ Tensor grad_norm(const Tensors& grads, int64_t stacked) {
   const at::NoGradGuard no_grad;
   check_grads(grads, stacked);
   if (grads.empty() || !grads[0].is_cuda()) return plain_norms(grads, stacked).to(at::kFloat);
+  check_no_trace("grad_norm");
   for (const Tensor& g : grads) check_no_tangent(g, "grad_norm");
   Tensors src;
   for (const Tensor& g : grads) src.push_back(dense(g, stacked) ? g : g.contiguous());
@@ -365,6 +378,7 @@ std::tuple<Tensors, Tensor> clip_grads(const Tensors& grads, double max_norm, in
     }
     return {out, norms.to(at::kFloat)};
   }
+  check_no_trace("clip_grads");
   for (const Tensor& g : grads) check_no_tangent(g, "clip_grads");
   // tensors without a common dense order go through contiguous copies; the kernels' entry point, which sees those instead of the
   // caller's memory, checks the lists that need none

@@ -7,7 +7,8 @@ they run the HIP kernels of libmgnn.so on the current stream, for float32, bfloa
 plain torch expression of the same formulas.  The checks, the autograd node and the memory are csrc/norm_torch.cpp, built as
 _norm_ops.so; a missing library raises.  What is not taken is refused with a TypeError (types, layouts) or a ValueError
 (shapes, sizes, devices, overlapping memory) before anything is written; what would lose its derivative, with a RuntimeError
-(NotImplementedError for forward-mode tangents, which the kernels do not carry).
+(NotImplementedError for forward-mode tangents, which the kernels do not carry, and while torch.jit.trace or make_fx
+records, which would not see the kernels).
 
 Nothing is kept between calls: workspaces come from torch's allocator, so every captured graph has its own.  As with any
 torch operator, a backward pass that is captured needs leaves whose eager graphs are gone.

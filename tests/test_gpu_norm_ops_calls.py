@@ -60,3 +60,20 @@ def test_forward_derivatives_are_refused():
     y = norm_ops.layer_norm(x, w, b)      # plain tensors in the same level
     assert forward_ad.unpack_dual(y).tangent is None
   assert torch.equal(norm_ops.layer_norm(x, w, b), y)
+
+
+def test_recording_a_trace_is_refused():
+  """A trace would record the outputs' allocation and not the kernels."""
+  from torch.fx.experimental.proxy_tensor import make_fx
+  x, w = normal((6, 20), 1), normal((20,), 2)
+  calls = (lambda t: norm_ops.layer_norm(t, w), lambda t: norm_ops.grad_norm([t]), lambda t: norm_ops.clip_grads([t], 0.5)[0][0])
+  for call in calls:
+    with pytest.raises(NotImplementedError, match='trace'):
+      torch.jit.trace(call, x, check_trace=False)
+    with pytest.raises(NotImplementedError, match='trace'):
+      make_fx(call)(x)
+    assert torch.isfinite(call(x)).all()
+  wg = w.clone().requires_grad_(True)
+  y = norm_ops.layer_norm(x, wg)
+  with pytest.raises(NotImplementedError, match='trace'):
+    make_fx(lambda dy: torch.autograd.grad(y, wg, dy, retain_graph=True)[0])(torch.ones_like(y))
