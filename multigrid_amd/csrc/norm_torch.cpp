@@ -304,6 +304,13 @@ void check_memory(const Tensors& grads, const Tensors& out) {
   }
 }
 
+// What these return has no graph: an input's would end there without a word
+void check_no_graph(const Tensors& grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor& g : grads)
+    TORCH_CHECK(!g.requires_grad(), what, " has no derivative, and one of the gradients requires grad: detach them or call it under torch.no_grad()");
+}
+
 std::vector<int64_t> norm_shape(int64_t stacked) { return stacked ? std::vector<int64_t>{stacked} : std::vector<int64_t>{}; }
 
 Tensor plain_norms(const Tensors& grads, int64_t stacked) {      // float64
@@ -341,8 +348,9 @@ Tensor launch(const Tensors& src, const Tensors* dst, double max_norm, int64_t s
 }
 
 Tensor grad_norm(const Tensors& grads, int64_t stacked) {
-  const at::NoGradGuard no_grad;
   check_grads(grads, stacked);
+  check_no_graph(grads, "grad_norm");
+  const at::NoGradGuard no_grad;
   if (grads.empty() || !grads[0].is_cuda()) return plain_norms(grads, stacked).to(at::kFloat);
   check_no_trace("grad_norm");
   for (const Tensor& g : grads) check_no_tangent(g, "grad_norm");
@@ -352,9 +360,10 @@ Tensor grad_norm(const Tensors& grads, int64_t stacked) {
 }
 
 std::tuple<Tensors, Tensor> clip_grads(const Tensors& grads, double max_norm, int64_t stacked, const std::optional<Tensors>& given) {
-  const at::NoGradGuard no_grad;
   check_grads(grads, stacked);
   TORCH_CHECK_VALUE(max_norm >= 0, "max_norm is a number >= 0, not ", max_norm);
+  if (!given) check_no_graph(grads, "clip_grads without out");
+  const at::NoGradGuard no_grad;
   const size_t count = grads.size();
   Tensors out;
   if (given) {

@@ -51,7 +51,8 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
 
 def grad_norm(grads, stacked=0):
   """The 2-norm of all gradients together, a float32 scalar on their device; stacked=A: every gradient has a leading
-  agent axis of A, and agent a's norm is element a of the result.  Squares are added in float64.  No gradients: 0."""
+  agent axis of A, and agent a's norm is element a of the result.  Squares are added in float64.  No gradients: 0.
+  It has no derivative: tensors that require grad are refused unless grad mode is off."""
   return (_EXT or load()).grad_norm([grads] if isinstance(grads, torch.Tensor) else list(grads), stacked)
 
 
@@ -59,14 +60,15 @@ def clip_grads(grads, max_norm, stacked=0, out=None):
   """([g * min(1, max_norm / (norm + 1e-6)) for every gradient g], norm) with norm = grad_norm(grads, stacked); agent by
   agent if stacked.  out: tensors of the gradients' shapes and types that receive the results, each its gradient itself (in
   place) or other memory; none of them may overlap itself, another result or another gradient of the call.  A norm that is
-  NaN makes every result NaN."""
+  NaN makes every result NaN.  It has no derivative: without out, tensors that require grad are refused unless grad mode is
+  off; out is written outside autograd, whatever graph the gradients carry."""
   return (_EXT or load()).clip_grads([grads] if isinstance(grads, torch.Tensor) else list(grads), max_norm, stacked,
                                      out if out is None else list(out))
 
 
 def clip_grad_norm_(parameters, max_norm, stacked=0):
   """torch.nn.utils.clip_grad_norm_ (v8_robust_ppo.py:340) on the parameters' .grad in place; parameters without one are
-  left out.  stacked=A: agent by agent.  Returns the norm(s) before clipping."""
+  left out.  stacked=A: agent by agent.  Returns the norm(s) before clipping.  Outside autograd, as torch's is."""
   parameters = [parameters] if isinstance(parameters, torch.Tensor) else parameters
   grads = [p.grad for p in parameters if p.grad is not None]
   return (_EXT or load()).clip_grads(grads, max_norm, stacked, grads)[1]

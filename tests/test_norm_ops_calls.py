@@ -1,5 +1,5 @@
 """Calls of multigrid_amd/norm_ops.py that must be refused or must not change what they return, on the CPU: memory that a
-clipping writes twice or reads after writing it."""
+clipping writes twice or reads after writing it, tensors whose graph would end in the call."""
 import itertools
 import random
 
@@ -86,3 +86,23 @@ def test_overlap_is_told_exactly():
     else:
       norm_ops.clip_grads(grads, 0.5, out=out)
   assert min(seen.values()) > 300
+
+
+def test_no_graph_is_cut_without_a_word():
+  """A norm, or results apart, of tensors that carry a graph would be constants to autograd."""
+  leaf = torch.ones(4, requires_grad=True)
+  for g in (leaf, leaf * 2):
+    with pytest.raises(RuntimeError, match='no derivative'):
+      norm_ops.grad_norm([torch.ones(3), g])
+    with pytest.raises(RuntimeError, match='no derivative'):
+      norm_ops.clip_grads([torch.ones(3), g], 0.5)
+    with torch.no_grad():
+      assert float(norm_ops.grad_norm(g)) == float(g.norm()) and len(norm_ops.clip_grads([g], 0.5)[0]) == 1
+    assert float(norm_ops.grad_norm([g.detach()])) == float(g.norm())
+  # in place and into given memory: outside autograd, as torch.nn.utils.clip_grad_norm_ is
+  p = torch.nn.Parameter(torch.ones(4))
+  p.square().sum().backward(create_graph=True)
+  assert p.grad.requires_grad and float(norm_ops.clip_grad_norm_([p], 0.5)) == 4.0
+  out = torch.zeros(4)
+  norm_ops.clip_grads([leaf * 2], 0.5, out=[out])
+  assert not out.requires_grad and torch.allclose(out, torch.full((4,), 0.25))
