@@ -77,3 +77,41 @@ def test_recording_a_trace_is_refused():
   y = norm_ops.layer_norm(x, wg)
   with pytest.raises(NotImplementedError, match='trace'):
     make_fx(lambda dy: torch.autograd.grad(y, wg, dy, retain_graph=True)[0])(torch.ones_like(y))
+
+
+@pytest.mark.parametrize('value', [1000.0, 4096.0, 30000.0, 1e10, 3.14159e-3, -77777.0])
+def test_rows_of_one_value_are_all_zero(value):
+  """Every deviation is 0, whatever the mean's rounding; and without eps 0 / 0."""
+  for cols in (1, 3, 7, 41, 60, 249, 255, 257, 1000, 1537, 2049, 5000, 9001, 16381):
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+      x = torch.full((3, cols), value, device='cuda').to(dtype)
+      if not torch.isfinite(x).all():
+        continue
+      bias = torch.full((cols,), 2.0, device='cuda')
+      xg, wg = x.clone().requires_grad_(True), torch.full((cols,), 3.0, device='cuda', requires_grad=True)
+      y = norm_ops.layer_norm(xg, wg, bias)
+      assert torch.equal(y, torch.full_like(y, 2.0)), (cols, dtype, float(y[0, 0].detach()))
+      dw, = torch.autograd.grad(y, wg, torch.ones_like(y))
+      assert not dw.any(), (cols, dtype, float(dw[0]))
+      assert torch.isnan(norm_ops.layer_norm(x, eps=0.0)).all(), (cols, dtype)
+
+
+@pytest.mark.parametrize('dtype', [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize('mean', [0.0, 300.0, -20000.0])
+def test_rows_off_centre_keep_their_deviations(mean, dtype):
+  """Deviations of 1 around a mean.  fp32: elements less a first mean m1, off by 40 u of 20000 at most, are exact; their own mean, below 0.9, is
+  off by 40 additions, 40 u; the sum of squares by 40 u relative, half of that in the root; x - m1 - shift, its product with
+  the root and the root itself by 4 u more.  Together 40 u + 24 u |h|, taken as 44 u (1 + |h|).  16 bits: the mean is rounded to fp32 besides,
+  and the result to its type."""
+  for cols in (5, 41, 128, 255, 513, 1537, 4100, 9001, 16381):
+    x = normal((23, cols), cols, mean, 1.0, dtype)
+    xd = x.double()
+    m = xd.mean(-1, keepdim=True)
+    rstd = 1 / torch.sqrt(((xd - m) ** 2).mean(-1, keepdim=True) + 1e-5)
+    want = (xd - m) * rstd
+    bound = 44 * U * (1 + want.abs())
+    if dtype != torch.float32:
+      bound += U * m.abs() * rstd
+      bound += (want.abs() + bound) * (torch.finfo(dtype).eps / 2) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    over = (norm_ops.layer_norm(x).double() - want).abs() - bound
+    assert float(over.max()) <= 0, (cols, float(over.max()))
