@@ -91,7 +91,6 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
     const Tensor stats = at::empty({s.groups * s.rows, 2}, x.options().dtype(at::kFloat));
     Tensor y = forward_kernel(rows, ld, x.sizes(), w, b, stats, eps, s);
     ctx->save_for_backward({rows, stats, w});
-    ctx->saved_data["ld"] = ld;
     ctx->saved_data["sizes"] = std::vector<int64_t>{s.groups, s.rows, s.cols, s.type, s.wtype};
     ctx->saved_data["affine"] = std::vector<int64_t>{weight.has_value(), bias.has_value(), weight ? weight->dim() : bias ? bias->dim() : 0};
     return y;
@@ -102,12 +101,19 @@ struct LayerNorm : public torch::autograd::Function<LayerNorm> {
     check_no_tangent(grads[0], "layer_norm's backward pass");
     check_no_trace("layer_norm's backward pass");
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &stats = saved[1], &w = saved[2];
-    const int64_t ld = ctx->saved_data["ld"].toInt();
     const auto n = ctx->saved_data["sizes"].toIntVector(), affine = ctx->saved_data["affine"].toIntVector();
     const Sizes s{n[0], n[1], n[2], (int)n[3], (int)n[4]};
-    const c10::DeviceGuard guard(x.device());
+    const c10::DeviceGuard guard(grads[0].device());
     const Tensor dy = grads[0].contiguous();
+    // hooks on saved tensors may give them back in other memory, with other strides
+    const auto as_saved = [&](const Tensor& t, int type, int64_t count) {
+      return t.device() == dy.device() && t.layout() == at::kStrided && type_of(t) == type && t.numel() == count;
+    };
+    TORCH_CHECK(as_saved(saved[0], s.type, s.groups * s.rows * s.cols) && as_saved(saved[1], MGNN_F32, s.groups * s.rows * 2) &&
+                    (!affine[0] || as_saved(saved[2], s.wtype, s.groups * s.cols)),
+                "layer_norm's saved tensors came back on another device, or of another type or size");
+    const auto [x, ld] = rows_of(saved[0], s.cols);
+    const Tensor stats = saved[1].contiguous(), w = affine[0] ? saved[2].contiguous() : Tensor();
     // the node's edges are those of the tensors that were given
     const bool want_w = affine[0] && ctx->needs_input_grad(1), want_b = affine[1] && ctx->needs_input_grad(affine[0] ? 2 : 1);
     Tensor dx, dw, db;

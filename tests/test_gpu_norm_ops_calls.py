@@ -115,3 +115,28 @@ def test_rows_off_centre_keep_their_deviations(mean, dtype):
       bound += (want.abs() + bound) * (torch.finfo(dtype).eps / 2) + torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
     over = (norm_ops.layer_norm(x).double() - want).abs() - bound
     assert float(over.max()) <= 0, (cols, float(over.max()))
+
+
+def test_saved_tensors_may_come_back_in_another_layout():
+  """Hooks on saved tensors (torch.autograd.graph.save_on_cpu) give back a contiguous copy of strided rows; other types, sizes or
+  devices are refused."""
+  wide = normal((50, 301), 1)
+  w, b, dy = normal((130,), 2), normal((130,), 3), normal((50, 130), 4)
+  for x in (wide[:, 7:137], wide[::2, 1:131].repeat(2, 1), normal((130, 50), 5).t()):
+    def grads(x, w, b):
+      xg, wg, bg = (t.detach().requires_grad_(True) for t in (x, w, b))
+      return norm_ops.layer_norm(xg, wg, bg), (xg, wg, bg)
+    y, leaves = grads(x, w, b)
+    want = torch.autograd.grad(y, leaves, dy)
+    with torch.autograd.graph.save_on_cpu():
+      y, leaves = grads(x, w, b)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, leaves, dy), want))
+    # rows that come back further apart than they left
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: torch.cat([t, t], dim=-1)[..., :t.size(-1)]):
+      y, leaves = grads(x, w, b)
+    assert all(torch.equal(p, q) for p, q in zip(torch.autograd.grad(y, leaves, dy), want))
+    for unpack in (lambda t: t.cpu(), lambda t: t.half(), lambda t: t[:1]):
+      with torch.autograd.graph.saved_tensors_hooks(lambda t: t, unpack):
+        y, leaves = grads(x, w, b)
+      with pytest.raises(RuntimeError, match='saved'):
+        torch.autograd.grad(y, leaves, dy)
