@@ -452,7 +452,16 @@ __global__ __launch_bounds__(kJoinCols* kJoinSlices) void ln_join_kernel(const f
   }
 }
 
-int launched() { return hipGetLastError() == hipSuccess ? MGNN_OK : MGNN_ERR_LAUNCH; }
+// Enqueues a kernel.  The status is the launch's own: the thread's last error may be an older one, of another call.
+template <typename T>
+struct Same { using type = T; };
+template <typename... P>
+int launch(void (*kernel)(P...), dim3 grid, int block, hipStream_t stream, const typename Same<P>::type&... args) {
+  void* list[] = {const_cast<void*>(static_cast<const void*>(&args))...};
+  if (hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, dim3(block), list, 0, stream) == hipSuccess) return MGNN_OK;
+  (void)hipGetLastError();      // reported here
+  return MGNN_ERR_LAUNCH;
+}
 
 int elem_bytes(int type) { return type == MGNN_F32 ? 4 : type == MGNN_BF16 || type == MGNN_F16 ? 2 : 0; }
 
@@ -521,7 +530,7 @@ int check_ln(int64_t ld, int64_t groups, int64_t rows, int C, int type, int wtyp
 
 // calls f.template operator()<TPR, NV, FULL>() for the split of rows of C elements
 template <typename T, typename F>
-void with_split(const RowSplit& s, int C, F f) {
+int with_split(const RowSplit& s, int C, F f) {
   const bool full = C == s.tpr * s.nv * Pack<T>::V;
   switch (s.tpr * 8 + s.nv) {
     case 1 * 8 + 1: return full ? f.template operator()<1, 1, true>() : f.template operator()<1, 1, false>();
@@ -539,6 +548,7 @@ void with_split(const RowSplit& s, int C, F f) {
     case 1024 * 8 + 4:      // fp32 rows of more than 8192
       if constexpr (std::is_same_v<T, float>) return full ? f.template operator()<1024, 4, true>() : f.template operator()<1024, 4, false>();
   }
+  return MGNN_ERR_SHAPE;      // row_split gives no other
 }
 
 template <typename T>
@@ -546,9 +556,9 @@ struct LnFwd {
   const T* x; int64_t ld; const void *weight, *bias; int wtype; T* y; float2* stats; int64_t groups, rows, blocks; int C; float eps;
   hipStream_t stream;
   template <int TPR, int NV, bool FULL>
-  void operator()() {
-    hipLaunchKernelGGL((ln_fwd_kernel<T, TPR, NV, FULL>), dim3((unsigned)blocks, (unsigned)groups), dim3(Shape<TPR>::BLOCK), 0,
-                       stream, x, ld, weight, bias, wtype, y, stats, rows, C, eps);
+  int operator()() {
+    return launch(ln_fwd_kernel<T, TPR, NV, FULL>, dim3((unsigned)blocks, (unsigned)groups), Shape<TPR>::BLOCK, stream, x, ld, weight, bias,
+                  wtype, y, stats, rows, C, eps);
   }
 };
 
@@ -557,9 +567,9 @@ struct LnBwd {
   const T* x; int64_t ld; const T* dy; const void* weight; int wtype; const float2* stats; T* dx; float* partial;
   void *dweight, *dbias; int64_t groups, rows, blocks; int C; hipStream_t stream;
   template <int TPR, int NV, bool FULL>
-  void operator()() {
-    hipLaunchKernelGGL((ln_bwd_kernel<T, TPR, NV, FULL>), dim3((unsigned)blocks, (unsigned)groups), dim3(Shape<TPR>::BLOCK), 0, stream, x,
-                       ld, dy, weight, wtype, stats, dx, partial, dweight, dbias, rows, C);
+  int operator()() {
+    return launch(ln_bwd_kernel<T, TPR, NV, FULL>, dim3((unsigned)blocks, (unsigned)groups), Shape<TPR>::BLOCK, stream, x, ld, dy, weight, wtype,
+                  stats, dx, partial, dweight, dbias, rows, C);
   }
 };
 
@@ -943,8 +953,7 @@ int clip(const void* const* src, void* const* dst, const int64_t* n, const int32
   if (int rc = grad_plan(src, dst, n, type, count, groups, plan)) return rc;
   if (!norms || (count > 0 && (!src || (max_norm >= 0 && !dst)))) return MGNN_ERR_VALUE;
   if (plan.tables.empty()) {
-    hipLaunchKernelGGL(zero_norms_kernel, dim3(1), dim3(256), 0, stream, norms, (int)groups);
-    return launched();
+    return launch(zero_norms_kernel, dim3(1), 256, stream, norms, (int)groups);
   }
   if (dst && overlaps(src, dst, n, type, count, groups)) return MGNN_ERR_OVERLAP;
   if (plan.slots) {
@@ -961,28 +970,24 @@ int clip(const void* const* src, void* const* dst, const int64_t* n, const int32
              : plan.slots == 12 ? grad_small_kernel<12, F> : grad_small_kernel<kSmallSlots, F>;
     };
     const auto kernel = floats ? pick(std::true_type()) : pick(std::false_type());
-    hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(kSmallBlock), 0, stream, t, dst ? max_norm : -1.0, norms);
-    return launched();
+    return launch(kernel, dim3((unsigned)groups), kSmallBlock, stream, t, dst ? max_norm : -1.0, norms);
   }
   if (!workspace || (uintptr_t)workspace % 8 || workspace_bytes < plan.workspace(groups)) return MGNN_ERR_WORKSPACE;
   double* partial = static_cast<double*>(workspace);
   int row = 0;
   for (size_t k = 0; k < plan.tables.size(); ++k) {
-    hipLaunchKernelGGL(grad_squares_kernel, dim3(plan.blocks[k], (unsigned)groups), dim3(kBlock), 0, stream, plan.tables[k], partial, row,
-                       plan.rows);
+    if (int rc = launch(grad_squares_kernel, dim3(plan.blocks[k], (unsigned)groups), kBlock, stream, plan.tables[k], partial, row, plan.rows))
+      return rc;
     row += plan.blocks[k];
   }
   int rows = plan.rows;
   if (rows > kMostRows) {
     double* sums = partial + rows * groups;
-    hipLaunchKernelGGL(grad_sum_kernel, dim3((unsigned)groups), dim3(1024), 0, stream, partial, rows, sums);
+    if (int rc = launch(grad_sum_kernel, dim3((unsigned)groups), 1024, stream, partial, rows, sums)) return rc;
     partial = sums;
     rows = 1;
   }
-  if (!dst) {
-    hipLaunchKernelGGL(grad_norm_kernel, dim3((unsigned)groups), dim3(kBlock), 0, stream, partial, rows, norms);
-    return launched();
-  }
+  if (!dst) return launch(grad_norm_kernel, dim3((unsigned)groups), kBlock, stream, partial, rows, norms);
   // Results of more than the 256 MB of the memory-side cache go past it: they would push out the gradients that are still
   // to be read, and the next reader would not find them there either (256 MB of bf16 apart: 153 -> 131 us, with a copy of
   // the results behind it 350 -> 348).
@@ -990,9 +995,10 @@ int clip(const void* const* src, void* const* dst, const int64_t* n, const int32
   for (int64_t i = 0; i < count; ++i) bytes += n[i] * groups * elem_bytes(type[i]);
   const bool past_caches = bytes >= (int64_t)256 << 20;
   for (size_t k = plan.tables.size(); k-- > 0;)
-    hipLaunchKernelGGL(grad_scale_kernel, dim3(plan.blocks[k], (unsigned)groups), dim3(kBlock), 0, stream, plan.tables[k], partial,
-                       rows, max_norm, k == 0 ? norms : nullptr, past_caches);
-  return launched();
+    if (int rc = launch(grad_scale_kernel, dim3(plan.blocks[k], (unsigned)groups), kBlock, stream, plan.tables[k], partial, rows, max_norm,
+                        k == 0 ? norms : nullptr, past_caches))
+      return rc;
+  return MGNN_OK;
 }
 
 }  // namespace
@@ -1007,13 +1013,11 @@ int mgnn_layer_norm(const void* x, int64_t ld, const void* weight, const void* b
   if (!x || !y) return MGNN_ERR_VALUE;
   auto go = [&](auto zero) {
     using T = decltype(zero);
-    with_split<T>(row_split(C, type), C, LnFwd<T>{static_cast<const T*>(x), ld, weight, bias, wtype, static_cast<T*>(y), reinterpret_cast<float2*>(stats),
-                                            groups, rows, forward_blocks(groups, rows, C, type), C, (float)eps, (hipStream_t)stream});
+    return with_split<T>(row_split(C, type), C, LnFwd<T>{static_cast<const T*>(x), ld, weight, bias, wtype, static_cast<T*>(y),
+                                                         reinterpret_cast<float2*>(stats), groups, rows, forward_blocks(groups, rows, C, type), C,
+                                                         (float)eps, (hipStream_t)stream});
   };
-  if (type == MGNN_F32) go(0.f);
-  else if (type == MGNN_BF16) go((__bf16)0.f);
-  else go((_Float16)0.f);
-  return launched();
+  return type == MGNN_F32 ? go(0.f) : type == MGNN_BF16 ? go((__bf16)0.f) : go((_Float16)0.f);
 }
 
 int64_t mgnn_layer_norm_workspace(int64_t groups, int64_t rows, int C, int type) {
@@ -1037,17 +1041,14 @@ int mgnn_layer_norm_backward(const void* x, int64_t ld, const void* dy, const vo
   float* partial = join ? static_cast<float*>(workspace) : nullptr;
   auto go = [&](auto zero) {
     using T = decltype(zero);
-    with_split<T>(row_split(C, type), C, LnBwd<T>{static_cast<const T*>(x), ld, static_cast<const T*>(dy), weight, wtype,
-                                            reinterpret_cast<const float2*>(stats), static_cast<T*>(dx), partial, dweight, dbias, groups,
-                                            rows, blocks, C, (hipStream_t)stream});
+    return with_split<T>(row_split(C, type), C, LnBwd<T>{static_cast<const T*>(x), ld, static_cast<const T*>(dy), weight, wtype,
+                                                         reinterpret_cast<const float2*>(stats), static_cast<T*>(dx), partial, dweight, dbias,
+                                                         groups, rows, blocks, C, (hipStream_t)stream});
   };
-  if (type == MGNN_F32) go(0.f);
-  else if (type == MGNN_BF16) go((__bf16)0.f);
-  else go((_Float16)0.f);
-  if (join)
-    hipLaunchKernelGGL(ln_join_kernel, dim3((unsigned)((2 * (int64_t)C + kJoinCols - 1) / kJoinCols), (unsigned)groups),
-                       dim3(kJoinCols * kJoinSlices), 0, (hipStream_t)stream, partial, (int)blocks, C, dweight, dbias, wtype);
-  return launched();
+  const int rc = type == MGNN_F32 ? go(0.f) : type == MGNN_BF16 ? go((__bf16)0.f) : go((_Float16)0.f);
+  if (rc || !join) return rc;
+  return launch(ln_join_kernel, dim3((unsigned)((2 * (int64_t)C + kJoinCols - 1) / kJoinCols), (unsigned)groups), kJoinCols * kJoinSlices,
+                (hipStream_t)stream, partial, (int)blocks, C, dweight, dbias, wtype);
 }
 
 int64_t mgnn_grad_norm_workspace(const int64_t* n, const int32_t* type, int64_t count, int64_t groups) try {

@@ -1,7 +1,11 @@
 """Calls of multigrid_amd/norm_ops.py on the GPU that must be refused, or that must return what simpler calls return."""
+import array
+import ctypes as C
+
 import pytest
 import torch
 
+import norm_abi
 from multigrid_amd import norm_ops
 
 pytestmark = pytest.mark.gpu
@@ -140,3 +144,22 @@ def test_saved_tensors_may_come_back_in_another_layout():
         y, leaves = grads(x, w, b)
       with pytest.raises(RuntimeError, match='saved'):
         torch.autograd.grad(y, leaves, dy)
+
+
+def test_an_older_error_of_the_thread_is_not_this_call_s():
+  """hipSetDevice of a device that is not there leaves an error behind; the calls after it succeed and say so."""
+  hip = C.CDLL('libamdhip64.so')
+  lib = norm_abi.load()
+  x, y, norm = normal((6, 20), 1), torch.zeros(6, 20, device='cuda'), torch.zeros(1, device='cuda')
+  n, t = array.array('q', [120]), array.array('i', [0])
+  src = array.array('Q', [x.data_ptr()])
+  stream = torch.cuda.current_stream().cuda_stream
+  torch.cuda.synchronize()
+  assert hip.hipSetDevice(12345) != 0
+  codes = [lib.mgnn_layer_norm(x.data_ptr(), 20, None, None, y.data_ptr(), None, 1, 6, 20, 1e-5, 0, 0, stream)]
+  assert hip.hipSetDevice(12345) != 0
+  codes.append(lib.mgnn_grad_norm(src.buffer_info()[0], n.buffer_info()[0], t.buffer_info()[0], 1, 1, norm.data_ptr(), None, 0, stream))
+  hip.hipGetLastError()
+  torch.cuda.synchronize()
+  assert codes == [0, 0]
+  assert torch.equal(y, norm_ops.layer_norm(x)) and torch.equal(norm[0], norm_ops.grad_norm([x]))
