@@ -75,5 +75,5 @@ def clip_grad_norm_(parameters, max_norm, stacked=0):
 
 
 def takes(grads):
-  """Whether grads, a list, are what the kernels take: tensors on a GPU, of the types they know."""
-  return bool(grads) and all(g.is_cuda and g.dtype in TYPES and g.layout is torch.strided for g in grads)
+  """Whether grads, a list, are what the kernels take: tensors on one GPU, of the types they know."""
+  return bool(grads) and all(g.is_cuda and g.device == grads[0].device and g.dtype in TYPES and g.layout is torch.strided for g in grads)

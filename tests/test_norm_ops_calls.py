@@ -2,6 +2,7 @@
 clipping writes twice or reads after writing it, tensors whose graph would end in the call."""
 import itertools
 import random
+import types
 
 import pytest
 import torch
@@ -106,3 +107,12 @@ def test_no_graph_is_cut_without_a_word():
   out = torch.zeros(4)
   norm_ops.clip_grads([leaf * 2], 0.5, out=[out])
   assert not out.requires_grad and torch.allclose(out, torch.full((4,), 0.25))
+
+
+def test_the_kernels_take_one_device():
+  """What the policies' clipping asks before it calls the kernels: a policy over several devices is left to torch."""
+  def grad(device='cuda:0', **kw):
+    return types.SimpleNamespace(**{'is_cuda': True, 'device': torch.device(device), 'dtype': torch.float32, 'layout': torch.strided, **kw})
+  assert norm_ops.takes([grad(), grad(dtype=torch.bfloat16)]) and norm_ops.takes([grad('cuda:1'), grad('cuda:1')])
+  assert not norm_ops.takes([grad(), grad('cuda:1')]) and not norm_ops.takes([]) and not norm_ops.takes([torch.ones(3)])
+  assert not norm_ops.takes([grad(), grad(dtype=torch.float64)]) and not norm_ops.takes([grad(layout=torch.sparse_coo)])
