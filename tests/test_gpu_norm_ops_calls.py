@@ -163,3 +163,70 @@ def test_an_older_error_of_the_thread_is_not_this_call_s():
   torch.cuda.synchronize()
   assert codes == [0, 0]
   assert torch.equal(y, norm_ops.layer_norm(x)) and torch.equal(norm[0], norm_ops.grad_norm([x]))
+
+
+def _leaves(x, w, b):
+  return tuple(t.detach().requires_grad_(True) for t in (x, w, b))
+
+
+SUMS = [(3, 409603, 128, torch.float32), (1, 300007, 64, torch.bfloat16), (2, 100003, 40, torch.bfloat16), (1, 958697, 35, torch.float32),
+        (1, 40001, 1024, torch.float16), (2, 5003, 2048, torch.bfloat16), (1, 5003, 1537, torch.float16), (5, 77, 8192, torch.float32),
+        (1, 2051, 16384, torch.float32), (1, 1031, 16381, torch.float32), (1, 509, 16384, torch.bfloat16), (70, 1001, 7, torch.float16)]
+
+
+@pytest.mark.parametrize('agents,rows,cols,dtype', SUMS)
+def test_sums_over_rows_count_every_row_once(agents, rows, cols, dtype):
+  """Whole numbers, whose sums below 2^24 fp32 holds exactly in any order: dy is odd everywhere, so that every row that is
+  missed or counted twice shows.  Rows of a power of 2 of +-1 have mean 0 and variance 1, so that without eps h is x itself."""
+  gen = torch.Generator(device='cuda').manual_seed(rows)
+  whole = cols & (cols - 1) == 0
+  dy = torch.randint(0, 4, (agents, rows, cols), device='cuda', generator=gen, dtype=torch.int8) * 2 - 3
+  x = torch.randint(0, 2, (agents, rows, cols // 2), device='cuda', generator=gen, dtype=torch.int8) * 2 - 1
+  x = torch.cat([x, -x] + [torch.zeros_like(x[..., :1])] * (cols % 2), dim=-1)
+  leaves = _leaves(x.to(dtype), normal((agents, cols), 1), normal((agents, cols), 2))
+  y = norm_ops.layer_norm(*leaves, eps=0.0)
+  _, dw, db = torch.autograd.grad(y, leaves, dy.to(dtype))
+  assert torch.equal(db.long(), dy.sum(-2, dtype=torch.int64)) and torch.equal(db, db.round())
+  if whole:
+    assert torch.equal(dw.long(), (dy * x).sum(-2, dtype=torch.int64)) and torch.equal(dw, dw.round())
+
+
+@pytest.mark.parametrize('agents,rows,cols,dtype', SUMS)
+def test_a_few_rows_of_many_carry_the_gradient(agents, rows, cols, dtype):
+  """dy is 0 but in 24 rows, the first and the last ones among them: sums of 24 terms, to which zeros add nothing.  A sum's terms
+  are off by h's error and its own by 24 roundings.  h = (x - m) s: m off by 40 u of the mean |x|, s by 24 u, two operations."""
+  x, w, b = normal((agents, rows, cols), 1, 0.4, 1.7, dtype), normal((agents, cols), 2), normal((agents, cols), 3)
+  at = torch.cat([torch.arange(8), torch.arange(8) * (rows // 9) + rows // 9 + 1, torch.arange(rows - 8, rows)]).unique().cuda()
+  few = normal((agents, len(at), cols), 4, 0, 1, dtype)
+  dy = torch.zeros(agents, rows, cols, dtype=dtype, device='cuda')
+  dy[:, at] = few
+  leaves = _leaves(x, w, b)
+  dx, dw, db = torch.autograd.grad(norm_ops.layer_norm(*leaves), leaves, dy)
+  xd, d = x[:, at].double(), few.double()
+  m = xd.mean(-1, keepdim=True)
+  s = 1 / torch.sqrt(((xd - m) ** 2).mean(-1, keepdim=True) + 1e-5)
+  h = (xd - m) * s
+  dh = 40 * U * xd.abs().mean(-1, keepdim=True) * s + 26 * U * h.abs()
+  terms = d * h
+  assert ((dw.double() - terms.sum(-2)).abs() <= ((24 * U) * terms.abs() + d.abs() * dh).sum(-2) * 1.01).all()
+  assert ((db.double() - d.sum(-2)).abs() <= 24 * U * d.abs().sum(-2) * 1.01).all()
+  dx[:, at] = 0
+  assert not dx.any()
+
+
+@pytest.mark.parametrize('agents,rows,cols,dtype,deep', [(3, 409603, 128, torch.float32, 302), (1, 100003, 40, torch.bfloat16, 4)])
+def test_sums_over_many_rows_of_real_numbers(agents, rows, cols, dtype, deep):
+  """deep: the rows one after the other in a thread, (rows / 8 to a step) over 170 workgroups and (rows / 32) over 782; then at most 3 steps
+  over lanes, 2 over waves, 25 and 5 over the workgroups' shares, each a rounding of the sum so far."""
+  x, dy = normal((agents, rows, cols), 1, 0.2, 1.0, dtype), normal((agents, rows, cols), 2, 0.1, 1, dtype)
+  leaves = _leaves(x, normal((agents, cols), 3, 1.0, 0.2), normal((agents, cols), 4))
+  _, dw, db = torch.autograd.grad(norm_ops.layer_norm(*leaves), leaves, dy)
+  for a in range(agents):
+    xd, d = x[a].double(), dy[a].double()
+    m = xd.mean(-1, keepdim=True)
+    s = 1 / torch.sqrt(((xd - m) ** 2).mean(-1, keepdim=True) + 1e-5)
+    h = (xd - m) * s
+    dh = 40 * U * xd.abs().mean(-1, keepdim=True) * s + 26 * U * h.abs()
+    terms, steps = d * h, (deep + 36) * U
+    assert ((dw[a].double() - terms.sum(-2)).abs() <= (steps * terms.abs() + d.abs() * dh).sum(-2)).all()
+    assert ((db[a].double() - d.sum(-2)).abs() <= steps * d.abs().sum(-2)).all()
