@@ -1,7 +1,8 @@
 // Layer norm with its gradients, and clipping by the global gradient norm (include/mgrid_norm.h): the normalisation of the
 // PPO trainer's policies and of their gradients.  Both are bound by HBM traffic; every element is moved 16 bytes per lane.
 // Rows and gradients may start at any element: gfx950 loads and stores 16 bytes at any address of an element's alignment,
-// so a row of odd length takes the same path as an even one, with its last, shorter vector element by element.
+// so a row of odd length takes the same path as an even one: its last vector ends at its end and overlaps the one before.
+// Rows shorter than one vector move element by element, and so does the last, shorter vector of a gradient.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -205,7 +206,7 @@ __device__ __forceinline__ float divide(float sum, float n, float inv_n) {
 // Where a row's elements lie close together, far from 0, the first mean's roundings are large beside their deviations (and all
 // there is of them in a row of equal values).  In 16 bits such elements add up exactly in fp32, a wave's 1024 at most, and the
 // quotient is rounded once.  In 32 bits the deviations from the first mean, which are exact there, are added up once more:
-// 3 x 4096 rows of 128 4.27 -> 4.43 us, 509 of 16381 15.4 -> 15.9, 3 x 409600 of 128 as before (226); 16-bit rows 0 to 1 %.
+// 3 x 4096 rows of 128 4.27 -> 4.43 us, 509 of 16381 15.4 -> 15.9, 3 x 409600 of 128 as before (226); 16-bit rows 0 to 2 %.
 // n, inv_n: the wave's elements of the row.  Rows over several waves: each wave's own mean m_w and deviations M_w, combined as
 // M = sum of M_w + n_w (m_w - m)^2, which takes one barrier instead of two; `origin` is the first wave's first mean.
 template <typename T, int TPR, int NV, bool FULL>
@@ -244,8 +245,8 @@ __device__ __forceinline__ void row_stats(const float (&v)[NV * Pack<T>::V], con
   }
 }
 
-// y = (x - m) s w + b.  Bound by HBM, each element read once and written once: 3 x 409600 rows of 128 fp32 219 us (5.7 TB/s),
-// 16384 of 4096 bf16 45 us (5.9); at 3 x 4096 rows of 128 fp32 4.2 us, a launch and one trip to memory.
+// y = (x - m) s w + b.  Bound by HBM, each element read once and written once: 3 x 409600 rows of 128 fp32 222 us (5.7 TB/s),
+// 16384 of 4096 bf16 46 us (5.8); at 3 x 4096 rows of 128 fp32 4.2 us, a launch and one trip to memory.
 template <typename T, int TPR, int NV, bool FULL>
 __global__ __launch_bounds__(Shape<TPR>::BLOCK) void ln_fwd_kernel(const T* x, int64_t ld, const void* weight, const void* bias,
                                                                    int wtype, T* y, float2* stats, int64_t rows, int C, float eps) {
@@ -315,8 +316,8 @@ __device__ __forceinline__ void slots_sum(float (&acc)[NE], float* lds) {
 }
 
 // dx = s (e - mean(e) - h mean(e h)) with e = dy w, and the sums of dy h and dy over this workgroup's rows.  Bound by HBM, x
-// and dy read once, dx written once: 3 x 409600 rows of 128 fp32 366 us (5.2 TB/s), 16384 of 4096 bf16 86 us (4.7); 509 rows
-// of 16381 fp32, two to a workgroup, 31 us, a quarter of the traffic shares.
+// and dy read once, dx written once: 3 x 409600 rows of 128 fp32 370 us (5.1 TB/s), 16384 of 4096 bf16 86 us (4.7); 509 rows
+// of 16381 fp32, four to each of 128 workgroups, 31 us (3.8 TB/s), a seventh of the traffic shares.
 // partial: [groups][blocks][2][C] floats (this workgroup's shares of dweight and dbias), or NULL with one block per group:
 // then dweight / dbias are written here
 template <typename T, int TPR, int NV, bool FULL>
@@ -426,7 +427,7 @@ __global__ __launch_bounds__(Shape<TPR>::BLOCK) void ln_bwd_kernel(const T* x, i
 
 // dweight / dbias of group blockIdx.y from the workgroups' shares, in a fixed order: 32 columns x 32 slices of the blocks,
 // sixteen loads in flight a thread.  4.5 to 5 us at up to 1024 shares of a few thousand columns, most of it a launch and two
-// trips to memory; 8.3 us for 256 shares of 2 x 16381 (4.0 TB/s).
+// trips to memory; 8.3 us for 128 shares of 2 x 16381 (2.0 TB/s): each thread's four loads are in flight at once, and then none.
 constexpr int kJoinCols = 32, kJoinSlices = 32;
 static_assert(kJoinCols == kJoinSlices);      // the transposed read
 __global__ __launch_bounds__(kJoinCols* kJoinSlices) void ln_join_kernel(const float* partial, int blocks, int C, void* dweight,
@@ -507,10 +508,14 @@ int64_t forward_blocks(int64_t groups, int64_t rows, int C, int type) {
   return want * groups <= 2048 * 256 / block ? want : even_blocks(want, groups, most);
 }
 
-// Backward: each workgroup leaves one row of shares of dweight and dbias to be added up, so there are fewer, the more so
-// the longer the rows, and each takes at least four steps.  fp32 3 x 409600 x 128, 512 / 768 / 1536 workgroups: 355 / 350 /
-// 383 us; bf16 3 x 409600 x 64: 97 / 92 / 96; 16384 x 4096: 83 / 93 / 107; 8192 columns (512 threads), 256 / 512: 56 / 67; half-
-// empty fp32 958698 x 35, 512 / 1024 / 1280: 129 / 86 / 81.
+// Backward: each workgroup leaves one row of shares of dweight and dbias to be added up, so there are fewer, the more so the longer
+// the rows.  fp32 3 x 409600 x 128, 512 / 768 / 1536 workgroups: 355 / 350 / 383 us; bf16 3 x 409600 x 64: 97 / 92 / 96, and 704 / 768
+// 93.4 / 93.2, 409600 x 512 235 / 240; 16384 x 4096, 512 / 768 / 1536: 83 / 93 / 107; 8192 columns (512 threads), 256 / 512: 56 / 67;
+// half-empty fp32 958698 x 35, 512 / 1024 / 1280: 129 / 86 / 81.
+// Each takes at least four steps, even where that leaves CUs idle: fewer shares are worth more.  With and without that minimum,
+// the join included: 509 x 16381 fp32 128 / 255 workgroups 43.4 / 47.8 us, 512 x 4096 bf16 128 / 512: 14.6 / 24.5, 256 x 8192 bf16
+// 64 / 256: 19.2 / 22.7, 2000 x 512 bf16 125 / 500: 8.4 / 11.6, 1024 x 1024 fp32 128 / 512: 9.8 / 10.2.  A pass for dx alone, which leaves
+// no shares, takes the same workgroups, and there the minimum costs: 27.9 / 24.6, 5.9 / 3.7, 6.9 / 3.7, 4.1 / 2.8, 4.9 / 3.2.
 int64_t backward_blocks(int64_t groups, int64_t rows, int C, int type) {
   const RowSplit s = row_split(C, type);
   const int64_t block = block_of(s), slots = block / s.tpr, want = (rows + slots - 1) / slots;
@@ -700,7 +705,7 @@ __device__ __forceinline__ void chunk_scale(const T* p, T* q, int64_t n, float f
   }
 }
 
-// Every workgroup adds up the partial sums itself (16 KB at most, from the caches) rather than waiting for a launch between.
+// Every workgroup adds up the partial sums itself (16 KB a table of the list, 128 KB at most, from the caches) rather than waiting for a launch between.
 // 2.1 GB of fp32 read and written in 767 us (5.6 TB/s), bound by HBM.
 __global__ __launch_bounds__(kBlock, 8) void grad_scale_kernel(GradTable t, const double* partial, int rows_of_group, double max_norm,
                                                             float* norms, bool past_caches) {
@@ -727,8 +732,12 @@ __global__ __launch_bounds__(kBlock, 8) void grad_scale_kernel(GradTable t, cons
 // Norms and clipping of gradients that one workgroup per group holds in its registers, SLOTS vectors of 16 bytes a thread:
 // one launch, and every element is read once.  The list's vectors are numbered through (t.end: vectors up to and with a
 // tensor); a tensor's last vector ends at its end and overlaps the one before, which counts the common elements; both
-// write the same values.  37544 fp32 in 13 tensors take 8.2 us, all on one CU: the table and each vector's tensor 0.9, loading
-// 1.5, fp64 squares 1.9, the norm 0.6, scaling and storing 2.7; two launches over many CUs take 4.4 + 5.1.  FLOATS: all of the
+// write the same values.  37544 fp32 in 13 tensors take 8.1 us, all on one CU: the table and each vector's tensor 0.9, loading
+// 1.5, fp64 squares 1.9, the norm 0.6, scaling and storing 2.7.
+// The limit is what the registers hold, and not where two launches over many CUs begin to win.  Called from the host, for which the
+// second launch is the dearer one, that is near it, written in place, one launch and two: 37544 fp32 8.5 and 11 us a call, 50544 in 16
+// tensors 10.7 and 11.8, 64800 12.7 and 11.1.  In a replayed graph it is at about 27000: 15996 4.8 and 6.2 us, 30000 6.8 and 6.6, 50544
+// 10.6 and 7.1, 129996 bf16 18.4 and 7.1.  FLOATS: all of the
 // list is fp32.  max_norm < 0: the norms alone.
 constexpr int kSmallBlock = 1024;
 constexpr int kSmallSlots = 16;      // at most: 64 of the 128 registers a thread of 1024 has
