@@ -7,6 +7,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
+#include <c10/util/SmallVector.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
@@ -242,7 +243,7 @@ class Sums {
       if (--tries_ < 0 || search(n - 1, total - i * t.step, t.below, t.every)) return true;
     return false;
   }
-  std::vector<Term> terms_;
+  c10::SmallVector<Term, 8> terms_;
   int64_t tries_ = 0;
 };
 
@@ -293,8 +294,9 @@ void check_memory(const Tensors& grads, const Tensors& out) {
   std::vector<Place> places;
   for (size_t i = 0; i < out.size(); ++i) {
     const Tensor &o = out[i], &g = grads[i];
-    // tensors without memory of their own: those of the meta device, and stand-ins for others
-    if (o.numel() == 0 || o.key_set().has(c10::DispatchKey::Meta) || g.key_set().has(c10::DispatchKey::Meta)) continue;
+    // without memory of their own: tensors of the meta device, and those that Python classes stand for (fake tensors)
+    const auto none = [](const Tensor& t) { return t.is_meta() || t.key_set().has(c10::DispatchKey::Python); };
+    if (o.numel() == 0 || none(o) || none(g)) continue;
     TORCH_CHECK_VALUE(!overlaps_itself(o), "a gradient that is written has several elements at one address (it overlaps itself)");
     places.push_back(place_of(o, i, true));
     if (!g.is_same(o)) places.push_back(place_of(g, i, false));

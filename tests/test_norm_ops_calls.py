@@ -116,3 +116,12 @@ def test_the_kernels_take_one_device():
   assert norm_ops.takes([grad(), grad(dtype=torch.bfloat16)]) and norm_ops.takes([grad('cuda:1'), grad('cuda:1')])
   assert not norm_ops.takes([grad(), grad('cuda:1')]) and not norm_ops.takes([]) and not norm_ops.takes([torch.ones(3)])
   assert not norm_ops.takes([grad(), grad(dtype=torch.float64)]) and not norm_ops.takes([grad(layout=torch.sparse_coo)])
+
+
+def test_fake_tensors_have_no_memory_to_overlap():
+  from torch._subclasses.fake_tensor import FakeTensorMode
+  with FakeTensorMode():
+    grads = [torch.ones(4), torch.ones(3, 3).t(), torch.ones(4)]
+    out, norm = norm_ops.clip_grads(grads, 0.5, out=grads)
+    assert norm.shape == () and [o.shape for o in out] == [g.shape for g in grads]
+    assert norm_ops.layer_norm(torch.ones(3, 4)).shape == (3, 4) and norm_ops.grad_norm(grads, 0).shape == ()
